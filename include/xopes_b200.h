@@ -345,6 +345,72 @@ LA_API int la_normalize_gate_bwd(const void *x, const void *gate, const float *w
                                  int64_t rows, int64_t G, int64_t e, int dtype, int act, int gate_pos,
                                  float c, float eps, int use_mean, void *stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Norms of queries and keys for each head, with the position rotation in the same pass: the op in front of
+ * lightning attention in a model block.  Per row (token, head) of D features, in fp32:
+ *     y = c * x / sqrt(sum x^2 + eps) * weight       (the norm of la_normalize_gate_fwd, weight (D) shared by heads)
+ *     out = y with the pairs of its first R features rotated by position * inv_freq[pair]
+ * q (B,N,H,D) and k (B,N,HK,D) of `dtype` by element strides of batch, token and head, features next to
+ * each other; outputs, their gradients, dq and dk contiguous.  Pairs are (i, i + R/2), interleaved != 0: (2i, 2i+1).
+ * Positions: positions[b*pos_sb + n*pos_sn] (int64, device memory), else n, or with cu_seqlens (M + 1 entries, B = 1)
+ * the place in the document; + offset.  inv_freq: R/2 doubles in HOST memory, radians per position, read before
+ * the call returns.  Weights (NULL: 1) are weight_dtype: LA_F32 or `dtype`.  D <= 512, R even, R <= D.
+ * The backward writes dq, dk (dtype) and, where not NULL, the weights' gradients (weight_dtype; summed in a fixed
+ * order through the workspace: la_qk_norm_rope_bwd_workspace_bytes(D) bytes, 4-byte aligned).
+ * ------------------------------------------------------------------------------------------- */
+LA_API int la_qk_norm_rope_fwd(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh, const void *k, int64_t k_sb,
+                               int64_t k_sn, int64_t k_sh, const void *q_weight, const void *k_weight,
+                               int weight_dtype, const int64_t *positions, int64_t pos_sb, int64_t pos_sn,
+                               int64_t offset, const int64_t *cu_seqlens, int64_t M, const double *inv_freq,
+                               void *q_out, void *k_out, int64_t B, int64_t N, int64_t H, int64_t HK, int64_t D,
+                               int64_t R, int dtype, int interleaved, float c, float eps, void *stream);
+LA_API int64_t la_qk_norm_rope_bwd_workspace_bytes(int64_t D);
+LA_API int la_qk_norm_rope_bwd(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh, const void *k, int64_t k_sb,
+                               int64_t k_sn, int64_t k_sh, const void *q_weight, const void *k_weight,
+                               int weight_dtype, const int64_t *positions, int64_t pos_sb, int64_t pos_sn,
+                               int64_t offset, const int64_t *cu_seqlens, int64_t M, const double *inv_freq,
+                               const void *d_q_out, const void *d_k_out, void *dq, void *dk, void *dq_weight,
+                               void *dk_weight, void *workspace, int64_t workspace_bytes, int64_t B, int64_t N,
+                               int64_t H, int64_t HK, int64_t D, int64_t R, int dtype, int interleaved, float c,
+                               float eps, void *stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Projections with what follows them: the ops behind lightning attention in a model block.  x (M,K) with row
+ * stride ldx, weights (N,K) with row stride ldw (elements, >= K; features next to each other), everything of
+ * `dtype`; outputs contiguous.  act: 0 none, 1 relu, 2 sigmoid, 3 silu, 4 gelu (by erf).
+ *     la_linear_fwd        z = x W^T + bias;  y = act(z) + residual          (bias, residual may be NULL)
+ *     la_gated_linear_fwd  g = x Wg^T + b_gate, u = x Wu^T + b_up;  h = act(g) u
+ * z (M,N) resp. gu (M,2N: g, then u) receive what the backward reads, or are NULL.  Accumulation in fp32, one
+ * rounding after the whole epilogue.
+ *     la_linear_bwd        dz = d_y act'(z);  dx = dz W, dweight = dz^T x, dbias = sum over rows of dz
+ *     la_gated_linear_bwd  dg = d_h u act'(g), du = d_h act(g);  dx = dg Wg + du Wu, dw_* , db_* as above
+ * Outputs that are NULL are skipped (dw_gate and dw_up only together).  dz, dg and du are rounded to `dtype`.
+ * z may be NULL without an activation.  Sums are taken in a fixed order: equal calls give equal bits.
+ * Workspace: la_linear_*_workspace_bytes for the same pointers (looked at for their alignment only), sizes and
+ * strides; weight_up NULL for the single projection; 16-byte aligned.  0: none needed; negative: LA_ERR_*.
+ * ------------------------------------------------------------------------------------------- */
+LA_API int64_t la_linear_fwd_workspace_bytes(const void *x, int64_t ldx, const void *weight, int64_t ldw,
+                                             const void *weight_up, int64_t ldw_up, int64_t M, int64_t N, int64_t K,
+                                             int dtype);
+LA_API int la_linear_fwd(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias,
+                         const void *residual, int64_t ldr, void *y, void *z, void *workspace,
+                         int64_t workspace_bytes, int64_t M, int64_t N, int64_t K, int dtype, int act, void *stream);
+LA_API int la_gated_linear_fwd(const void *x, int64_t ldx, const void *w_gate, int64_t ld_gate, const void *w_up,
+                               int64_t ld_up, const void *b_gate, const void *b_up, void *h, void *gu,
+                               void *workspace, int64_t workspace_bytes, int64_t M, int64_t N, int64_t K, int dtype,
+                               int act, void *stream);
+LA_API int64_t la_linear_bwd_workspace_bytes(const void *x, int64_t ldx, const void *weight, int64_t ldw,
+                                             const void *weight_up, int64_t ldw_up, const void *d_y, int64_t ldy,
+                                             int64_t M, int64_t N, int64_t K, int dtype, int act, int want_dx,
+                                             int want_dw, int want_db);
+LA_API int la_linear_bwd(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *z,
+                         const void *d_y, int64_t ldy, void *dx, void *dweight, void *dbias, void *workspace,
+                         int64_t workspace_bytes, int64_t M, int64_t N, int64_t K, int dtype, int act, void *stream);
+LA_API int la_gated_linear_bwd(const void *x, int64_t ldx, const void *w_gate, int64_t ld_gate, const void *w_up,
+                               int64_t ld_up, const void *gu, const void *d_h, int64_t ldh, void *dx, void *dw_gate,
+                               void *dw_up, void *db_gate, void *db_up, void *workspace, int64_t workspace_bytes,
+                               int64_t M, int64_t N, int64_t K, int dtype, int act, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

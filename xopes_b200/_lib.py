@@ -63,6 +63,24 @@ SIGNATURES = {
                                      _i32, _vp]),
     "la_normalize_gate_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32,
                                      _i32, _f32, _f32, _i32, _vp]),
+    "la_qk_norm_rope_fwd": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _i64,
+                                   _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32,
+                                   _f32, _f32, _vp]),
+    "la_qk_norm_rope_bwd_workspace_bytes": (_i64, [_i64]),
+    "la_qk_norm_rope_bwd": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _i64,
+                                   _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
+                                   _i64, _i64, _i32, _i32, _f32, _f32, _vp]),
+    "la_linear_fwd_workspace_bytes": (_i64, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i32]),
+    "la_linear_fwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _i32,
+                             _vp]),
+    "la_gated_linear_fwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
+                                   _i32, _i32, _vp]),
+    "la_linear_bwd_workspace_bytes": (_i64, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _i32,
+                                             _i32, _i32, _i32]),
+    "la_linear_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32,
+                             _i32, _vp]),
+    "la_gated_linear_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
+                                   _i64, _i64, _i64, _i32, _i32, _vp]),
     "la_decode_scalar": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp,
                                 _i64, _i64, _i64, _i64, _i32, _vp]),
     "la_decode_vector": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,

@@ -1,0 +1,629 @@
+// linear_fn and gated_linear_fn: the host plan of both directions, the fp32 product, and the passes around the
+// matrix products (derivative of the activation, sums over rows, sums over the splits of a contraction).
+//
+//   linear        z = x W^T + b             y = act(z) + r
+//                 dz = dy act'(z)           dx = dz W      dW = dz^T x      db = sum over rows of dz
+//   gated pair    g = x Wg^T + bg, u = x Wu^T + bu         h = act(g) u
+//                 dg = dh u act'(g), du = dh act(g)        dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, sums
+//
+// x (M, K), W (N, K).  Every product is accumulated in fp32 and rounded once, after bias, activation, product of
+// the pair and residual.  What the backward needs of the forward is z, or g and u, kept in the type of x (one rounding;
+// computing them again would cost a third of the forward's and backward's products together).  dz is rounded to the
+// type of x too, since it is an operand of two products.
+#include "linear.cuh"
+
+namespace la {
+namespace lin {
+
+int sm_count() {
+  static int sms[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    cudaGetLastError();
+    return 148;
+  }
+  if (sms[dev] == 0) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      return 148;
+    }
+    sms[dev] = n;
+  }
+  return sms[dev];
+}
+
+namespace {
+
+// ------------------------------------------------------------------------------ product on CUDA cores
+struct SimtArgs {
+  Operand a[2], b[2];
+  long long K[2];
+  int vec_a[2], vec_b[2];
+  int segments;
+  long long M, N;
+  int n_tiles, splits;
+  long long steps[2];  // 16-wide steps of each segment
+  float *partial;      // (splits, pair ? 2 : 1, M, N) or null
+  Epilogue e;
+};
+
+constexpr int kTile = 64, kStep = 16, kPitch = kTile + 4;
+
+// four elements of a 64 x 16 operand tile for this thread: along the contraction, or along the rows (mn_major)
+template <typename T>
+__device__ __forceinline__ void simt_fetch(const Operand &o, int vec, long long r0, long long R, long long k0, long long K,
+                                           float (&v)[4]) {
+  const int t = threadIdx.x;
+  const T *p = static_cast<const T *>(o.p);
+  if (!o.mn_major) {
+    const long long r = r0 + (t >> 2), k = k0 + (t & 3) * 4;
+    if (r < R) load_row<T, 4>(p + r * o.ld + k, vec, (int)(K - k < 4 ? K - k : 4), v);
+    else v[0] = v[1] = v[2] = v[3] = 0.f;
+  } else {
+    const long long k = k0 + (t >> 4), r = r0 + (t & 15) * 4;
+    if (k < K) load_row<T, 4>(p + k * o.ld + r, vec, (int)(R - r < 4 ? R - r : 4), v);
+    else v[0] = v[1] = v[2] = v[3] = 0.f;
+  }
+}
+__device__ __forceinline__ void simt_put(const Operand &o, float (*s)[kPitch], const float (&v)[4]) {
+  const int t = threadIdx.x;
+  if (!o.mn_major) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[(t & 3) * 4 + j][t >> 2] = v[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[t >> 4][(t & 15) * 4 + j] = v[j];
+  }
+}
+
+// One 64 x 64 tile (of one split) per CTA of 256 threads, 4 x 4 results a thread; the next step's operands are in
+// registers while the current step's are multiplied.
+template <typename T, bool PAIR>
+__global__ void __launch_bounds__(256) simt_product_kernel(const SimtArgs a) {
+  __shared__ __align__(16) float sa[kStep][kPitch], sb[PAIR ? 2 : 1][kStep][kPitch];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const long long tile = blockIdx.x / a.splits;
+  const int split = (int)(blockIdx.x - tile * a.splits);
+  const long long m0 = tile / a.n_tiles * kTile, n0 = tile % a.n_tiles * kTile;
+  const long long all = a.steps[0] + a.steps[1];
+  const long long s0 = all * split / a.splits, s1 = all * (split + 1) / a.splits;
+  float acc[4][4] = {}, acc2[PAIR ? 4 : 1][4] = {};
+  float va[4], vb[4], vb2[4];
+  auto fetch = [&](long long s) {
+    const int g = s >= a.steps[0];
+    const long long k0 = (g ? s - a.steps[0] : s) * kStep;
+    simt_fetch<T>(a.a[g], a.vec_a[g], m0, a.M, k0, a.K[g], va);
+    simt_fetch<T>(a.b[g], a.vec_b[g], n0, a.N, k0, a.K[g], vb);
+    if (PAIR) simt_fetch<T>(a.b[1], a.vec_b[1], n0, a.N, k0, a.K[0], vb2);
+  };
+  if (s0 < s1) fetch(s0);
+  for (long long s = s0; s < s1; ++s) {
+    const int g = s >= a.steps[0];
+    __syncthreads();
+    simt_put(a.a[g], sa, va);
+    simt_put(a.b[g], sb[0], vb);
+    if (PAIR) simt_put(a.b[1], sb[PAIR ? 1 : 0], vb2);
+    __syncthreads();
+    if (s + 1 < s1) fetch(s + 1);
+#pragma unroll
+    for (int k = 0; k < kStep; ++k) {
+      const float4 x = *reinterpret_cast<const float4 *>(&sa[k][ty * 4]);
+      const float4 y = *reinterpret_cast<const float4 *>(&sb[0][k][tx * 4]);
+      const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] += xs[i] * ys[j];
+      if (PAIR) {
+        const float4 z = *reinterpret_cast<const float4 *>(&sb[PAIR ? 1 : 0][k][tx * 4]);
+        const float zs[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc2[PAIR ? i : 0][j] += xs[i] * zs[j];
+      }
+    }
+  }
+  const long long n = n0 + tx * 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const long long m = m0 + ty * 4 + i;
+    if (m >= a.M || n >= a.N) continue;
+    if (a.partial != nullptr) {
+      float *p = a.partial + ((long long)split * (PAIR ? 2 : 1) * a.M + m) * a.N + n;
+      const int left = (int)(a.N - n < 4 ? a.N - n : 4);
+      store_row<float, 4>(p, a.N % 4 == 0, left, acc[i]);
+      if (PAIR) store_row<float, 4>(p + a.M * a.N, a.N % 4 == 0, left, acc2[PAIR ? i : 0]);
+    } else if (PAIR) {
+      finish_pair<T, 4>(a.e, m, (int)n, (int)a.N, acc[i], acc2[PAIR ? i : 0]);
+    } else {
+      finish_one<T, 4>(a.e, m, (int)n, (int)a.N, acc[i]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------ sums over the splits
+// out of the partial products (splits, PAIR ? 2 : 1, M, N) in a fixed order, then the epilogue; 8 columns a thread
+template <typename T, bool PAIR>
+__global__ void __launch_bounds__(256) split_sum_kernel(const float *partial, int splits, long long M, int N, Epilogue e) {
+  constexpr int W = 8;
+  const int packs = (N + W - 1) / W;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= M * packs) return;
+  const long long m = i / packs;
+  const int n = (int)(i - m * packs) * W, left = N - n;
+  const bool vec = N % 4 == 0;
+  const long long mat = M * N;
+  float g[W] = {}, u[W] = {};
+  const float *p = partial + m * N + n;
+  for (int s = 0; s < splits; ++s) {
+    float v[W];
+    load_row<float, W>(p, vec, left, v);
+#pragma unroll
+    for (int j = 0; j < W; ++j) g[j] += v[j];
+    p += mat;
+    if (PAIR) {
+      load_row<float, W>(p, vec, left, v);
+#pragma unroll
+      for (int j = 0; j < W; ++j) u[j] += v[j];
+      p += mat;
+    }
+  }
+  if (PAIR) finish_pair<T, W>(e, m, n, N, g, u);
+  else finish_one<T, W>(e, m, n, N, g);
+}
+
+// ------------------------------------------------------------------------------ derivative of the activation
+struct ActGradArgs {
+  const void *dy, *z;       // (M, N) and, for a pair, g and u of z at columns 0 and z_up
+  long long ldy, ldz;
+  int z_up;
+  void *dz;                 // or null: only the sums
+  long long ldd;
+  int d_up;
+  float *partial;           // (chunks, PAIR ? 2N : N) sums over the chunk's rows, or null
+  long long M, N;
+  long long rows;           // rows of a chunk
+  int act;
+};
+
+// CTA = 32 x VEC columns of one chunk of rows, a warp per row at a time.  One read of dy and z, one write of dz: HBM.
+template <typename T, int VEC, bool PAIR>
+__global__ void __launch_bounds__(256) act_grad_kernel(const ActGradArgs a) {
+  __shared__ float part[PAIR ? 2 : 1][8][32 * VEC + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long n = ((long long)blockIdx.x * 32 + lane) * VEC;
+  const int left = a.N - n < VEC ? (int)(a.N - n) : VEC;
+  const long long r0 = (long long)blockIdx.y * a.rows, r1 = r0 + a.rows < a.M ? r0 + a.rows : a.M;
+  float s0[VEC] = {}, s1[VEC] = {};
+  if (left > 0) {
+#pragma unroll 2
+    for (long long m = r0 + warp; m < r1; m += 8) {
+      float dy[VEC], z[VEC], u[VEC], du[VEC];
+      load_row<T, VEC>(static_cast<const T *>(a.dy) + m * a.ldy + n, VEC > 1, left, dy);
+      if (a.z != nullptr) load_row<T, VEC>(static_cast<const T *>(a.z) + m * a.ldz + n, VEC > 1, left, z);
+      if (PAIR) load_row<T, VEC>(static_cast<const T *>(a.z) + m * a.ldz + a.z_up + n, VEC > 1, left, u);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        float act = 0.f;
+        const float d = a.z != nullptr ? act_grad_of<T>(z[j], a.act, act) : 1.f;
+        if (PAIR) {
+          du[j] = dy[j] * act;
+          dy[j] = dy[j] * u[j] * d;
+          s1[j] += du[j];
+        } else {
+          dy[j] *= d;
+        }
+        s0[j] += dy[j];
+      }
+      if (a.dz != nullptr) {
+        T *o = static_cast<T *>(a.dz) + m * a.ldd + n;
+        store_row<T, VEC>(o, VEC > 1, left, dy);
+        if (PAIR) store_row<T, VEC>(o + a.d_up, VEC > 1, left, du);
+      }
+    }
+  }
+  if (a.partial == nullptr) return;  // uniform over the grid
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    part[0][warp][lane * VEC + j] = s0[j];
+    if (PAIR) part[PAIR ? 1 : 0][warp][lane * VEC + j] = s1[j];
+  }
+  __syncthreads();
+  const long long width = PAIR ? 2 * a.N : a.N;
+  for (int c = threadIdx.x; c < 32 * VEC; c += 256) {
+    const long long col = (long long)blockIdx.x * 32 * VEC + c;
+    if (col >= a.N) break;
+    float v0 = 0.f, v1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      v0 += part[0][w][c];
+      if (PAIR) v1 += part[PAIR ? 1 : 0][w][c];
+    }
+    a.partial[blockIdx.y * width + col] = v0;
+    if (PAIR) a.partial[blockIdx.y * width + a.N + col] = v1;
+  }
+}
+
+// db[c] = sum over the chunks, in a fixed order.  Columns from N on belong to the second bias.
+template <typename T>
+__global__ void __launch_bounds__(256) bias_sum_kernel(const float *partial, int chunks, long long width, long long N,
+                                                       void *db0, void *db1) {
+  __shared__ float s[8][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const long long c = (long long)blockIdx.x * 32 + tx;
+  float v = 0.f;
+  if (c < width)
+    for (int i = ty; i < chunks; i += 8) v += partial[i * width + c];
+  s[ty][tx] = v;
+  __syncthreads();
+  if (ty != 0 || c >= width) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) v += s[i][tx];
+  T *db = static_cast<T *>(c < N ? db0 : db1);
+  if (db != nullptr) db[c < N ? c : c - N] = Cvt<T>::from_f(v);
+}
+
+// ------------------------------------------------------------------------------ host
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Scratch in pieces out of the caller's workspace; with base null it only counts.
+struct Scratch {
+  char *base;
+  int64_t used = 0;
+  explicit Scratch(void *p) : base(static_cast<char *>(p)) {}
+  void *take(int64_t bytes) {
+    void *p = base == nullptr ? nullptr : base + used;
+    used += (bytes + 255) / 256 * 256;
+    return p;
+  }
+};
+
+int epilogue_vec(const Epilogue &e, int dtype) {
+  const int64_t per = 16 / (int64_t)dtype_size(dtype);
+  return aligned16(e.bias[0]) && aligned16(e.bias[1]) && aligned16(e.residual) && aligned16(e.out) && aligned16(e.out2) &&
+         aligned16(e.save) && e.ldr % per == 0 && e.ldo % per == 0 && e.lds % per == 0 && e.save_up % per == 0;
+}
+
+template <typename T>
+int simt_launch(const Product &p, int splits, float *partial, cudaStream_t st) {
+  SimtArgs a = {};
+  a.segments = p.segments;
+  a.M = p.M; a.N = p.N; a.e = p.e;
+  for (int s = 0; s < 2; ++s) {
+    a.a[s] = p.a[s]; a.b[s] = p.b[s];
+    a.K[s] = s < p.segments ? p.K[s] : 0;
+    a.steps[s] = (a.K[s] + kStep - 1) / kStep;
+    a.vec_a[s] = aligned16(p.a[s].p) && p.a[s].ld % 4 == 0;
+    a.vec_b[s] = aligned16(p.b[s].p) && p.b[s].ld % 4 == 0;
+  }
+  const int64_t mt = (p.M + kTile - 1) / kTile;
+  a.n_tiles = (int)((p.N + kTile - 1) / kTile);
+  a.splits = splits;
+  a.partial = partial;
+  const int64_t grid = mt * a.n_tiles * splits;
+  if (grid > INT32_MAX) return LA_ERR_TOO_LARGE;
+  if (p.pair) simt_product_kernel<T, true><<<(unsigned)grid, 256, 0, st>>>(a);
+  else simt_product_kernel<T, false><<<(unsigned)grid, 256, 0, st>>>(a);
+  return launch_status();
+}
+
+template <typename T>
+int split_sum_launch(const Product &p, int splits, const float *partial, cudaStream_t st) {
+  const int64_t grid = (p.M * ((p.N + 7) / 8) + 255) / 256;
+  if (grid > INT32_MAX) return LA_ERR_TOO_LARGE;
+  if (p.pair) split_sum_kernel<T, true><<<(unsigned)grid, 256, 0, st>>>(partial, splits, p.M, (int)p.N, p.e);
+  else split_sum_kernel<T, false><<<(unsigned)grid, 256, 0, st>>>(partial, splits, p.M, (int)p.N, p.e);
+  return launch_status();
+}
+
+// One product with its epilogue.  With s.base null only the scratch is counted.
+int product(Product p, int dtype, Scratch s, int64_t &need, cudaStream_t st) {
+  const int64_t k = p.K[0] + (p.segments > 1 ? p.K[1] : 0);
+  const int64_t tiles = (p.M + kTile - 1) / kTile * ((p.N + kTile - 1) / kTile);
+  int64_t splits = 2 * (int64_t)sm_count() / tiles;  // two CTAs per SM at least, 128 terms a split at least
+  if (splits > k / 128) splits = k / 128;
+  if (splits > 16) splits = 16;
+  if (splits < 1) splits = 1;
+  float *partial = nullptr;
+  if (splits > 1) partial = static_cast<float *>(s.take(splits * (p.pair ? 2 : 1) * p.M * p.N * 4));
+  if (s.used > need) need = s.used;
+  if (s.base == nullptr) return LA_OK;
+  p.e.vec = epilogue_vec(p.e, dtype);
+  int rc = LA_ERR_UNSUPPORTED;
+  switch (dtype) {
+    case LA_F32: rc = simt_launch<float>(p, (int)splits, partial, st); break;
+    case LA_BF16: rc = simt_launch<__nv_bfloat16>(p, (int)splits, partial, st); break;
+    case LA_F16: rc = simt_launch<__half>(p, (int)splits, partial, st); break;
+  }
+  if (rc != LA_OK || partial == nullptr) return rc;
+  switch (dtype) {
+    case LA_F32: return split_sum_launch<float>(p, (int)splits, partial, st);
+    case LA_BF16: return split_sum_launch<__nv_bfloat16>(p, (int)splits, partial, st);
+    case LA_F16: return split_sum_launch<__half>(p, (int)splits, partial, st);
+  }
+  return LA_ERR_UNSUPPORTED;
+}
+
+template <typename T, int VEC>
+void act_grad_launch(const ActGradArgs &a, bool pair, int chunks, cudaStream_t st) {
+  const dim3 grid((unsigned)((a.N + 32 * VEC - 1) / (32 * VEC)), (unsigned)chunks);
+  if (pair) act_grad_kernel<T, VEC, true><<<grid, 256, 0, st>>>(a);
+  else act_grad_kernel<T, VEC, false><<<grid, 256, 0, st>>>(a);
+}
+
+// chunks of rows of act_grad_kernel: four CTAs per SM, at least 8 rows (one per warp) a chunk
+int act_grad_chunks(int64_t M, int64_t N, int dtype) {
+  const int64_t cols = 32 * (16 / (int64_t)dtype_size(dtype));
+  int64_t chunks = 8 * (int64_t)sm_count() / ((N + cols - 1) / cols);
+  if (chunks > (M + 7) / 8) chunks = (M + 7) / 8;
+  if (chunks > 4096) chunks = 4096;
+  return chunks < 1 ? 1 : (int)chunks;
+}
+
+int act_grad(ActGradArgs a, bool pair, int chunks, void *db0, void *db1, int dtype, cudaStream_t st) {
+  a.rows = (a.M + chunks - 1) / chunks;
+  const int64_t per = 16 / (int64_t)dtype_size(dtype);
+  const bool vec = aligned16(a.dy) && aligned16(a.z) && aligned16(a.dz) && a.ldy % per == 0 && a.ldz % per == 0 &&
+                   a.ldd % per == 0 && a.z_up % per == 0 && a.d_up % per == 0;
+  switch (dtype) {
+    case LA_F32: vec ? act_grad_launch<float, 4>(a, pair, chunks, st) : act_grad_launch<float, 1>(a, pair, chunks, st); break;
+    case LA_BF16:
+      vec ? act_grad_launch<__nv_bfloat16, 8>(a, pair, chunks, st) : act_grad_launch<__nv_bfloat16, 1>(a, pair, chunks, st);
+      break;
+    case LA_F16: vec ? act_grad_launch<__half, 8>(a, pair, chunks, st) : act_grad_launch<__half, 1>(a, pair, chunks, st); break;
+  }
+  int rc = launch_status();
+  if (rc != LA_OK || a.partial == nullptr) return rc;
+  const int64_t width = pair ? 2 * a.N : a.N;
+  const unsigned grid = (unsigned)((width + 31) / 32);
+  switch (dtype) {
+    case LA_F32: bias_sum_kernel<float><<<grid, 256, 0, st>>>(a.partial, chunks, width, a.N, db0, db1); break;
+    case LA_BF16: bias_sum_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a.partial, chunks, width, a.N, db0, db1); break;
+    case LA_F16: bias_sum_kernel<__half><<<grid, 256, 0, st>>>(a.partial, chunks, width, a.N, db0, db1); break;
+  }
+  return launch_status();
+}
+
+struct FwdArgs {
+  const void *x;
+  int64_t ldx;
+  const void *w[2];
+  int64_t ldw[2];
+  const void *bias[2], *residual;
+  int64_t ldr;
+  void *out, *save;
+  int64_t M, N, K;
+  int dtype, act, pair;
+};
+
+int forward(const FwdArgs &f, Scratch s, int64_t &need, cudaStream_t st) {
+  Product p = {};
+  p.a[0] = Operand{f.x, f.ldx, 0};
+  p.b[0] = Operand{f.w[0], f.ldw[0], 0};
+  p.b[1] = Operand{f.w[1], f.ldw[1], 0};
+  p.K[0] = f.K;
+  p.segments = 1;
+  p.pair = f.pair;
+  p.M = f.M; p.N = f.N;
+  p.e.bias[0] = f.bias[0]; p.e.bias[1] = f.bias[1];
+  p.e.residual = f.residual; p.e.ldr = f.ldr;
+  p.e.out = f.out; p.e.ldo = f.N; p.e.split = INT32_MAX; p.e.live = (int)f.M;
+  p.e.save = f.save; p.e.lds = f.pair ? 2 * f.N : f.N; p.e.save_up = f.pair ? (int)f.N : 0;
+  p.e.act = f.act;
+  return product(p, f.dtype, s, need, st);
+}
+
+struct BwdArgs {
+  const void *x;
+  int64_t ldx;
+  const void *w[2];
+  int64_t ldw[2];
+  const void *saved, *dy;
+  int64_t ldy;
+  void *dx, *dw[2], *db[2];
+  int64_t M, N, K;
+  int dtype, act, pair;
+};
+
+int backward(const BwdArgs &f, Scratch s, int64_t &need, cudaStream_t st) {
+  const bool run = s.base != nullptr;
+  const int64_t es = (int64_t)dtype_size(f.dtype);
+  const bool want_dw = f.dw[0] != nullptr, want_db = f.db[0] != nullptr || f.db[1] != nullptr;
+  const bool products = f.dx != nullptr || want_dw;
+  // dz: dy itself without an activation, else a pass of its own; dg and du side by side, each on a 16-byte boundary
+  const int64_t np = (f.N + 7) / 8 * 8;
+  const bool own_dz = f.pair || f.act != kActNone;
+  Operand dz = {f.dy, f.ldy, 0};
+  if (own_dz && products) dz = Operand{s.take(f.M * (f.pair ? 2 * np : np) * es), f.pair ? 2 * np : np, 0};
+  const int chunks = act_grad_chunks(f.M, f.N, f.dtype);
+  float *sums = want_db ? static_cast<float *>(s.take((int64_t)chunks * (f.pair ? 2 : 1) * f.N * 4)) : nullptr;
+  int rc;
+  if (run && ((own_dz && products) || want_db)) {
+    ActGradArgs a = {};
+    a.dy = f.dy; a.ldy = f.ldy;
+    if (own_dz) {
+      a.z = f.saved;
+      a.ldz = f.pair ? 2 * f.N : f.N;
+      a.z_up = f.pair ? (int)f.N : 0;
+    }
+    if (own_dz && products) {
+      a.dz = const_cast<void *>(dz.p);
+      a.ldd = dz.ld;
+      a.d_up = f.pair ? (int)np : 0;
+    }
+    a.partial = sums;
+    a.M = f.M; a.N = f.N; a.act = f.act;
+    if ((rc = act_grad(a, f.pair != 0, chunks, f.db[0], f.db[1], f.dtype, st)) != LA_OK) return rc;
+  }
+  const void *dz_up = dz.p == nullptr ? nullptr : static_cast<const char *>(dz.p) + np * es;
+  if (f.dx != nullptr) {
+    Product p = {};
+    p.a[0] = dz;
+    p.a[1] = Operand{dz_up, dz.ld, 0};
+    p.b[0] = Operand{f.w[0], f.ldw[0], 1};
+    p.b[1] = Operand{f.w[1], f.ldw[1], 1};
+    p.K[0] = f.N; p.K[1] = f.pair ? f.N : 0;
+    p.segments = f.pair ? 2 : 1;
+    p.M = f.M; p.N = f.K;
+    p.e.out = f.dx; p.e.ldo = f.K; p.e.split = INT32_MAX; p.e.live = (int)f.M;
+    if ((rc = product(p, f.dtype, s, need, st)) != LA_OK) return rc;
+  }
+  if (want_dw) {
+    Product p = {};
+    p.a[0] = Operand{dz.p, dz.ld, 1};
+    p.b[0] = Operand{f.x, f.ldx, 1};
+    p.K[0] = f.M;
+    p.segments = 1;
+    p.M = f.pair ? np + f.N : f.N;  // a pair: rows [0, N) are dWg, rows [np, np + N) dWu
+    p.N = f.K;
+    p.e.out = f.dw[0]; p.e.out2 = f.dw[1]; p.e.ldo = f.K;
+    p.e.split = f.pair ? (int)np : (int)f.N;
+    p.e.live = (int)f.N;
+    if ((rc = product(p, f.dtype, s, need, st)) != LA_OK) return rc;
+  }
+  if (s.used > need) need = s.used;
+  return LA_OK;
+}
+
+int check_common(int64_t M, int64_t N, int64_t K, int dtype, int act) {
+  cudaGetLastError();
+  if (M <= 0 || N <= 0 || K <= 0) return LA_ERR_BAD_SHAPE;
+  if (!(dtype == LA_F32 || dtype == LA_BF16 || dtype == LA_F16)) return LA_ERR_UNSUPPORTED;
+  if (act < kActNone || act > kActGelu) return LA_ERR_UNSUPPORTED;
+  if (M > (1 << 30) || N > (1 << 28) || K > (1 << 28)) return LA_ERR_TOO_LARGE;
+  return LA_OK;
+}
+
+int check_fwd(const FwdArgs &f) {
+  if (f.x == nullptr || f.w[0] == nullptr || (f.pair && f.w[1] == nullptr)) return LA_ERR_NULL_POINTER;
+  const int rc = check_common(f.M, f.N, f.K, f.dtype, f.act);
+  if (rc != LA_OK) return rc;
+  if (f.ldx < f.K || f.ldw[0] < f.K || (f.pair && f.ldw[1] < f.K) || (f.residual != nullptr && f.ldr < f.N))
+    return LA_ERR_BAD_SHAPE;
+  return LA_OK;
+}
+int check_bwd(const BwdArgs &f) {
+  if (f.x == nullptr || f.w[0] == nullptr || (f.pair && f.w[1] == nullptr) || f.dy == nullptr) return LA_ERR_NULL_POINTER;
+  const int rc = check_common(f.M, f.N, f.K, f.dtype, f.act);
+  if (rc != LA_OK) return rc;
+  if ((f.pair || f.act != kActNone) && f.saved == nullptr) return LA_ERR_NULL_POINTER;
+  if (f.pair && (f.dw[0] == nullptr) != (f.dw[1] == nullptr)) return LA_ERR_NULL_POINTER;
+  if (f.ldx < f.K || f.ldw[0] < f.K || (f.pair && f.ldw[1] < f.K) || f.ldy < f.N) return LA_ERR_BAD_SHAPE;
+  return LA_OK;
+}
+
+int check_scratch(int64_t need, void *workspace, int64_t workspace_bytes) {
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return LA_ERR_WORKSPACE;
+  if (need > 0 && !aligned16(workspace)) return LA_ERR_MISALIGNED;
+  return LA_OK;
+}
+
+// a base for calls that need no scratch: never read, only told apart from the counting run
+char g_no_scratch[16];
+
+int run_fwd(const FwdArgs &f, void *workspace, int64_t workspace_bytes, void *stream) {
+  int rc = check_fwd(f);
+  if (rc != LA_OK) return rc;
+  if (f.out == nullptr) return LA_ERR_NULL_POINTER;
+  int64_t need = 0;
+  rc = forward(f, Scratch(nullptr), need, nullptr);  // counts the scratch
+  if (rc == LA_OK) rc = check_scratch(need, workspace, workspace_bytes);
+  if (rc != LA_OK) return rc;
+  return forward(f, Scratch(need > 0 ? workspace : g_no_scratch), need, static_cast<cudaStream_t>(stream));
+}
+int run_bwd(const BwdArgs &f, void *workspace, int64_t workspace_bytes, void *stream) {
+  int rc = check_bwd(f);
+  if (rc != LA_OK) return rc;
+  int64_t need = 0;
+  rc = backward(f, Scratch(nullptr), need, nullptr);
+  if (rc == LA_OK) rc = check_scratch(need, workspace, workspace_bytes);
+  if (rc != LA_OK) return rc;
+  return backward(f, Scratch(need > 0 ? workspace : g_no_scratch), need, static_cast<cudaStream_t>(stream));
+}
+
+}  // namespace
+}  // namespace lin
+}  // namespace la
+
+using namespace la;
+using namespace la::lin;
+
+extern "C" {
+
+int64_t la_linear_fwd_workspace_bytes(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *weight_up,
+                                      int64_t ldw_up, int64_t M, int64_t N, int64_t K, int dtype) {
+  FwdArgs f = {};
+  f.x = x; f.ldx = ldx;
+  f.w[0] = weight; f.ldw[0] = ldw; f.w[1] = weight_up; f.ldw[1] = ldw_up;
+  f.M = M; f.N = N; f.K = K; f.dtype = dtype; f.pair = weight_up != nullptr;
+  int64_t need = 0;
+  const int rc = check_fwd(f);
+  if (rc != LA_OK) return rc;
+  forward(f, Scratch(nullptr), need, nullptr);
+  return need;
+}
+
+int la_linear_fwd(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, const void *residual,
+                  int64_t ldr, void *y, void *z, void *workspace, int64_t workspace_bytes, int64_t M, int64_t N, int64_t K,
+                  int dtype, int act, void *stream) {
+  FwdArgs f = {};
+  f.x = x; f.ldx = ldx; f.w[0] = weight; f.ldw[0] = ldw; f.bias[0] = bias;
+  f.residual = residual; f.ldr = residual == nullptr ? 0 : ldr;
+  f.out = y; f.save = z; f.M = M; f.N = N; f.K = K; f.dtype = dtype; f.act = act;
+  return run_fwd(f, workspace, workspace_bytes, stream);
+}
+
+int la_gated_linear_fwd(const void *x, int64_t ldx, const void *w_gate, int64_t ld_gate, const void *w_up, int64_t ld_up,
+                        const void *b_gate, const void *b_up, void *h, void *gu, void *workspace, int64_t workspace_bytes,
+                        int64_t M, int64_t N, int64_t K, int dtype, int act, void *stream) {
+  FwdArgs f = {};
+  f.x = x; f.ldx = ldx; f.w[0] = w_gate; f.ldw[0] = ld_gate; f.w[1] = w_up; f.ldw[1] = ld_up;
+  f.bias[0] = b_gate; f.bias[1] = b_up;
+  f.out = h; f.save = gu; f.M = M; f.N = N; f.K = K; f.dtype = dtype; f.act = act; f.pair = 1;
+  return run_fwd(f, workspace, workspace_bytes, stream);
+}
+
+int64_t la_linear_bwd_workspace_bytes(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *weight_up,
+                                      int64_t ldw_up, const void *d_y, int64_t ldy, int64_t M, int64_t N, int64_t K,
+                                      int dtype, int act, int want_dx, int want_dw, int want_db) {
+  static char any[16];  // stands for an output that is wanted
+  BwdArgs f = {};
+  f.x = x; f.ldx = ldx; f.w[0] = weight; f.ldw[0] = ldw; f.w[1] = weight_up; f.ldw[1] = ldw_up;
+  f.pair = weight_up != nullptr;
+  f.saved = any; f.dy = d_y; f.ldy = ldy;
+  f.dx = want_dx ? any : nullptr;
+  f.dw[0] = f.dw[1] = want_dw ? any : nullptr;
+  f.db[0] = want_db ? any : nullptr;
+  f.M = M; f.N = N; f.K = K; f.dtype = dtype; f.act = act;
+  int64_t need = 0;
+  const int rc = check_bwd(f);
+  if (rc != LA_OK) return rc;
+  backward(f, Scratch(nullptr), need, nullptr);
+  return need;
+}
+
+int la_linear_bwd(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *z, const void *d_y, int64_t ldy,
+                  void *dx, void *dweight, void *dbias, void *workspace, int64_t workspace_bytes, int64_t M, int64_t N,
+                  int64_t K, int dtype, int act, void *stream) {
+  BwdArgs f = {};
+  f.x = x; f.ldx = ldx; f.w[0] = weight; f.ldw[0] = ldw; f.saved = z; f.dy = d_y; f.ldy = ldy;
+  f.dx = dx; f.dw[0] = dweight; f.db[0] = dbias;
+  f.M = M; f.N = N; f.K = K; f.dtype = dtype; f.act = act;
+  return run_bwd(f, workspace, workspace_bytes, stream);
+}
+
+int la_gated_linear_bwd(const void *x, int64_t ldx, const void *w_gate, int64_t ld_gate, const void *w_up, int64_t ld_up,
+                        const void *gu, const void *d_h, int64_t ldh, void *dx, void *dw_gate, void *dw_up, void *db_gate,
+                        void *db_up, void *workspace, int64_t workspace_bytes, int64_t M, int64_t N, int64_t K, int dtype,
+                        int act, void *stream) {
+  BwdArgs f = {};
+  f.x = x; f.ldx = ldx; f.w[0] = w_gate; f.ldw[0] = ld_gate; f.w[1] = w_up; f.ldw[1] = ld_up;
+  f.saved = gu; f.dy = d_h; f.ldy = ldh;
+  f.dx = dx; f.dw[0] = dw_gate; f.dw[1] = dw_up; f.db[0] = db_gate; f.db[1] = db_up;
+  f.M = M; f.N = N; f.K = K; f.dtype = dtype; f.act = act; f.pair = 1;
+  return run_bwd(f, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,148 @@
+"""Norms of queries and keys for each head with the position rotation in the same pass: the op in front of
+lightning attention in a model block.
+
+    y   = c * x / sqrt(sum(x^2) + eps) * weight        per row (token, head), as in normalize_gate_fn
+    out = y with its first rotary_dim features rotated by position * inv_freq
+
+One CUDA pass over q and k each way.  c = sqrt(D) with eps = D * 1e-6 is the RMS norm with 1e-6, c = 1 the
+L2 norm.  The norm is normalize's without gate (xopes/ops/normalize/normalize/normalize_torch.py:9-111).
+"""
+import ctypes
+import functools
+from typing import Optional, Sequence, Tuple
+
+import torch
+
+from . import _lib
+
+
+@functools.lru_cache(maxsize=64)
+def _frequencies(base: float, rotary_dim: int):
+    """base^(-2i / rotary_dim) as the host array of doubles the C entry takes."""
+    n = rotary_dim // 2
+    return (ctypes.c_double * max(n, 1))(*[base ** (-2.0 * i / rotary_dim) for i in range(n)])
+
+
+class QkNormRopeFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, positions, offset, cu, freq, rotary_dim, interleaved, c, eps):
+        lib = _lib.load()
+        q, k = (t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous() for t in (q, k))
+        b, n, h, d = q.shape
+        hk = k.shape[2]
+        wq, wk, wcode = _weights(q, q_weight, k_weight)
+        qo = torch.empty(b, n, h, d, dtype=q.dtype, device=q.device)
+        ko = torch.empty(b, n, hk, d, dtype=q.dtype, device=q.device)
+        pos_sb, pos_sn = (0, 0) if positions is None else (positions.stride(0) if positions.shape[0] > 1 else 0,
+                                                           positions.stride(1))
+        m = 0 if cu is None else cu.numel() - 1
+        with _lib.device_of(q):
+            rc = lib.la_qk_norm_rope_fwd(
+                _lib.ptr(q), *q.stride()[:3], _lib.ptr(k), *k.stride()[:3], _lib.ptr(wq), _lib.ptr(wk), wcode,
+                _lib.ptr(positions), pos_sb, pos_sn, offset, _lib.ptr(cu), m, freq, _lib.ptr(qo), _lib.ptr(ko),
+                b, n, h, hk, d, rotary_dim, _lib.dtype_code(q), interleaved, c, eps, _lib.stream_of(q))
+        _lib.check(rc, "la_qk_norm_rope_fwd")
+        ctx.save_for_backward(q, k, q_weight, k_weight, positions, cu)
+        ctx.cfg = (offset, freq, rotary_dim, interleaved, c, eps, pos_sb, pos_sn)
+        ctx.set_materialize_grads(False)
+        return qo, ko
+
+    @staticmethod
+    def backward(ctx, dqo, dko):
+        lib = _lib.load()
+        q, k, q_weight, k_weight, positions, cu = ctx.saved_tensors
+        offset, freq, rotary_dim, interleaved, c, eps, pos_sb, pos_sn = ctx.cfg
+        b, n, h, d = q.shape
+        hk = k.shape[2]
+        dqo = torch.zeros(b, n, h, d, dtype=q.dtype, device=q.device) if dqo is None else dqo.to(q.dtype).contiguous()
+        dko = torch.zeros(b, n, hk, d, dtype=q.dtype, device=q.device) if dko is None else dko.to(q.dtype).contiguous()
+        wq, wk, wcode = _weights(q, q_weight, k_weight)
+        dq = torch.empty(b, n, h, d, dtype=q.dtype, device=q.device)
+        dk = torch.empty(b, n, hk, d, dtype=q.dtype, device=q.device)
+        dwq = torch.empty_like(wq) if wq is not None and ctx.needs_input_grad[2] else None
+        dwk = torch.empty_like(wk) if wk is not None and ctx.needs_input_grad[3] else None
+        ws, ws_bytes = None, 0
+        if dwq is not None or dwk is not None:
+            ws_bytes = lib.la_qk_norm_rope_bwd_workspace_bytes(d)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+        m = 0 if cu is None else cu.numel() - 1
+        with _lib.device_of(q):
+            rc = lib.la_qk_norm_rope_bwd(
+                _lib.ptr(q), *q.stride()[:3], _lib.ptr(k), *k.stride()[:3], _lib.ptr(wq), _lib.ptr(wk), wcode,
+                _lib.ptr(positions), pos_sb, pos_sn, offset, _lib.ptr(cu), m, freq, _lib.ptr(dqo), _lib.ptr(dko),
+                _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dwq), _lib.ptr(dwk), _lib.ptr(ws), ws_bytes,
+                b, n, h, hk, d, rotary_dim, _lib.dtype_code(q), interleaved, c, eps, _lib.stream_of(q))
+        _lib.check(rc, "la_qk_norm_rope_bwd")
+        return (dq, dk, None if dwq is None else dwq.to(q_weight.dtype), None if dwk is None else dwk.to(k_weight.dtype),
+                None, None, None, None, None, None, None, None)
+
+
+def _weights(q, q_weight, k_weight):
+    """The weights in one type the kernel reads: both of q's type, or fp32."""
+    given = [w.dtype for w in (q_weight, k_weight) if w is not None]
+    dt = q.dtype if given and all(t == q.dtype for t in given) else torch.float32
+    wq, wk = (None if w is None else w.detach().to(dt).contiguous() for w in (q_weight, k_weight))
+    return wq, wk, _lib.dtype_code(q) if dt == q.dtype else _lib.LA_F32
+
+
+def qk_norm_rope_fn(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                    k_weight: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, offset: int = 0,
+                    cu_seqlens: Optional[torch.LongTensor] = None, c: float = 1.0, eps: float = 1e-6,
+                    base: float = 10000.0, rotary_dim: Optional[int] = None,
+                    inv_freq: Optional[Sequence[float]] = None, interleaved: bool = False
+                    ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """q (B,N,H,D), k (B,N,HK,D), HK any number of key heads; any strides with the features next to each other
+    (slices of one projection need no copy).  Returns new contiguous tensors of the same shapes and type.
+    Gradients for q, k and the weights.
+
+    q_weight, k_weight: (D,), shared by the heads; None = 1.
+    positions: int64 (B,N), (1,N) or (N,); None counts from 0 in every sequence, or in every document of
+        cu_seqlens (M+1,) int64, batch 1.  offset is added (a host number; under a captured graph give positions).
+    rotary_dim: rotated features, the first of each head; even, D if None, 0 for the norm alone.
+    inv_freq: rotary_dim / 2 host numbers, radians per position; base^(-2i / rotary_dim) if None.
+    interleaved: pairs are features (2i, 2i+1) instead of (i, i + rotary_dim / 2).
+    D up to 512."""
+    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[-1] != k.shape[-1]:
+        raise ValueError(f"q (B,N,H,D) and k (B,N,HK,D) expected, got {tuple(q.shape)} and {tuple(k.shape)}")
+    if q.dtype != k.dtype:
+        raise TypeError(f"q and k must have one dtype, got {q.dtype} and {k.dtype}")
+    b, n, _, d = q.shape
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and tuple(w.shape) != (d,):
+            raise ValueError(f"{name} must have shape ({d},), got {tuple(w.shape)}")
+    r = d - d % 2 if rotary_dim is None else int(rotary_dim)
+    if r < 0 or r > d or r % 2:
+        raise ValueError(f"rotary_dim must be even and between 0 and {d}, got {rotary_dim}")
+    if inv_freq is None:
+        freq = _frequencies(float(base), r)
+    else:
+        if isinstance(inv_freq, torch.Tensor):
+            if inv_freq.is_cuda:
+                raise ValueError("inv_freq is read on the host: give numbers or a CPU tensor")
+            inv_freq = inv_freq.tolist()
+        if len(inv_freq) != r // 2:
+            raise ValueError(f"inv_freq must have {r // 2} entries, got {len(inv_freq)}")
+        freq = (ctypes.c_double * max(r // 2, 1))(*[float(f) for f in inv_freq])
+    if positions is not None:
+        if cu_seqlens is not None:
+            raise ValueError("give positions or cu_seqlens, not both")
+        if positions.dtype != torch.int64:
+            raise TypeError(f"positions must be int64, got {positions.dtype}")
+        if positions.dim() == 1:
+            positions = positions[None]
+        if positions.dim() != 2 or positions.shape[0] not in (1, b) or positions.shape[1] != n:
+            raise ValueError(f"positions must have shape ({b},{n}), (1,{n}) or ({n},), got {tuple(positions.shape)}")
+    _lib.require_cuda(q, k, q_weight, k_weight, positions, cu_seqlens)
+    for t in (k, q_weight, k_weight, positions, cu_seqlens):
+        if t is not None and t.device != q.device:
+            raise ValueError(f"all tensors must be on {q.device}, got one on {t.device}")
+    cu = None
+    if cu_seqlens is not None:
+        if b != 1:
+            raise AssertionError("cu_seqlens is only supported for batch size 1")
+        cu = cu_seqlens.to(torch.int64).contiguous()
+    _lib.dtype_code(q)
+    if q.numel() == 0 or k.numel() == 0:
+        raise ValueError("q and k must have at least one element")
+    return QkNormRopeFunction.apply(q, k, q_weight, k_weight, positions, int(offset), cu, freq, r, int(bool(interleaved)),
+                                    float(c), float(eps))
