@@ -380,8 +380,9 @@ LA_API int la_qk_norm_rope_bwd(const void *q, int64_t q_sb, int64_t q_sn, int64_
  * `dtype`; outputs contiguous.  act: 0 none, 1 relu, 2 sigmoid, 3 silu, 4 gelu (by erf).
  *     la_linear_fwd        z = x W^T + bias;  y = act(z) + residual          (bias, residual may be NULL)
  *     la_gated_linear_fwd  g = x Wg^T + b_gate, u = x Wu^T + b_up;  h = act(g) u
- * z (M,N) resp. gu (M,2N: g, then u) receive what the backward reads, or are NULL.  Accumulation in fp32, one
- * rounding after the whole epilogue.
+ * z resp. gu receive what the backward reads (pre-activations: fp32, or the upper 24 bits of fp32 for 16-bit types), or
+ * are NULL: la_linear_saved_bytes(M, N, dtype, pair) bytes, 16-byte aligned.  Accumulation in fp32, one
+ * rounding after the whole epilogue.  16-bit types run on the tensor cores, fp32 on the CUDA cores.
  *     la_linear_bwd        dz = d_y act'(z);  dx = dz W, dweight = dz^T x, dbias = sum over rows of dz
  *     la_gated_linear_bwd  dg = d_h u act'(g), du = d_h act(g);  dx = dg Wg + du Wu, dw_* , db_* as above
  * Outputs that are NULL are skipped (dw_gate and dw_up only together).  dz, dg and du are rounded to `dtype`.
@@ -389,6 +390,7 @@ LA_API int la_qk_norm_rope_bwd(const void *q, int64_t q_sb, int64_t q_sn, int64_
  * Workspace: la_linear_*_workspace_bytes for the same pointers (looked at for their alignment only), sizes and
  * strides; weight_up NULL for the single projection; 16-byte aligned.  0: none needed; negative: LA_ERR_*.
  * ------------------------------------------------------------------------------------------- */
+LA_API int64_t la_linear_saved_bytes(int64_t M, int64_t N, int dtype, int pair);
 LA_API int64_t la_linear_fwd_workspace_bytes(const void *x, int64_t ldx, const void *weight, int64_t ldw,
                                              const void *weight_up, int64_t ldw_up, int64_t M, int64_t N, int64_t K,
                                              int dtype);

@@ -70,6 +70,7 @@ SIGNATURES = {
     "la_qk_norm_rope_bwd": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i32, _vp, _i64, _i64, _i64,
                                    _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
                                    _i64, _i64, _i32, _i32, _f32, _f32, _vp]),
+    "la_linear_saved_bytes": (_i64, [_i64, _i64, _i32, _i32]),
     "la_linear_fwd_workspace_bytes": (_i64, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _i32]),
     "la_linear_fwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _i32,
                              _vp]),

@@ -7,9 +7,11 @@
 //                 dg = dh u act'(g), du = dh act(g)        dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, sums
 //
 // x (M, K), W (N, K).  Every product is accumulated in fp32 and rounded once, after bias, activation, product of
-// the pair and residual.  What the backward needs of the forward is z, or g and u, kept in the type of x (one rounding;
-// computing them again would cost a third of the forward's and backward's products together).  dz is rounded to the
-// type of x too, since it is an operand of two products.
+// the pair and residual.  What the backward needs of the forward is z, or g and u: for 16-bit types kept as the upper 24
+// bits of their fp32 values (computing them again would cost a third of the forward's and backward's products together; kept
+// in 16 bits their two roundings made the gradients of a pair 1.8 times as far off as rounding the gradients alone
+// does, in 24 bits 1.4 times, which is what the rounding of dz leaves).  dz is rounded to the type of x, since it is an
+// operand of two products.
 #include "linear.cuh"
 
 namespace la {
@@ -35,7 +37,7 @@ int sm_count() {
 
 namespace {
 
-// ------------------------------------------------------------------------------ product on CUDA cores
+// ------------------------------------------------------------------------------ fp32 product on the CUDA cores
 struct SimtArgs {
   Operand a[2], b[2];
   long long K[2];
@@ -51,18 +53,17 @@ struct SimtArgs {
 constexpr int kTile = 64, kStep = 16, kPitch = kTile + 4;
 
 // four elements of a 64 x 16 operand tile for this thread: along the contraction, or along the rows (mn_major)
-template <typename T>
 __device__ __forceinline__ void simt_fetch(const Operand &o, int vec, long long r0, long long R, long long k0, long long K,
                                            float (&v)[4]) {
   const int t = threadIdx.x;
-  const T *p = static_cast<const T *>(o.p);
+  const float *p = static_cast<const float *>(o.p);
   if (!o.mn_major) {
     const long long r = r0 + (t >> 2), k = k0 + (t & 3) * 4;
-    if (r < R) load_row<T, 4>(p + r * o.ld + k, vec, (int)(K - k < 4 ? K - k : 4), v);
+    if (r < R) load_row<float, 4>(p + r * o.ld + k, vec, (int)(K - k < 4 ? K - k : 4), v);
     else v[0] = v[1] = v[2] = v[3] = 0.f;
   } else {
     const long long k = k0 + (t >> 4), r = r0 + (t & 15) * 4;
-    if (k < K) load_row<T, 4>(p + k * o.ld + r, vec, (int)(R - r < 4 ? R - r : 4), v);
+    if (k < K) load_row<float, 4>(p + k * o.ld + r, vec, (int)(R - r < 4 ? R - r : 4), v);
     else v[0] = v[1] = v[2] = v[3] = 0.f;
   }
 }
@@ -79,7 +80,7 @@ __device__ __forceinline__ void simt_put(const Operand &o, float (*s)[kPitch], c
 
 // One 64 x 64 tile (of one split) per CTA of 256 threads, 4 x 4 results a thread; the next step's operands are in
 // registers while the current step's are multiplied.
-template <typename T, bool PAIR>
+template <bool PAIR>
 __global__ void __launch_bounds__(256) simt_product_kernel(const SimtArgs a) {
   __shared__ __align__(16) float sa[kStep][kPitch], sb[PAIR ? 2 : 1][kStep][kPitch];
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
@@ -93,9 +94,9 @@ __global__ void __launch_bounds__(256) simt_product_kernel(const SimtArgs a) {
   auto fetch = [&](long long s) {
     const int g = s >= a.steps[0];
     const long long k0 = (g ? s - a.steps[0] : s) * kStep;
-    simt_fetch<T>(a.a[g], a.vec_a[g], m0, a.M, k0, a.K[g], va);
-    simt_fetch<T>(a.b[g], a.vec_b[g], n0, a.N, k0, a.K[g], vb);
-    if (PAIR) simt_fetch<T>(a.b[1], a.vec_b[1], n0, a.N, k0, a.K[0], vb2);
+    simt_fetch(a.a[g], a.vec_a[g], m0, a.M, k0, a.K[g], va);
+    simt_fetch(a.b[g], a.vec_b[g], n0, a.N, k0, a.K[g], vb);
+    if (PAIR) simt_fetch(a.b[1], a.vec_b[1], n0, a.N, k0, a.K[0], vb2);
   };
   if (s0 < s1) fetch(s0);
   for (long long s = s0; s < s1; ++s) {
@@ -136,9 +137,9 @@ __global__ void __launch_bounds__(256) simt_product_kernel(const SimtArgs a) {
       store_row<float, 4>(p, a.N % 4 == 0, left, acc[i]);
       if (PAIR) store_row<float, 4>(p + a.M * a.N, a.N % 4 == 0, left, acc2[PAIR ? i : 0]);
     } else if (PAIR) {
-      finish_pair<T, 4>(a.e, m, (int)n, (int)a.N, acc[i], acc2[PAIR ? i : 0]);
+      finish_pair<float, 4>(a.e, m, (int)n, (int)a.N, acc[i], acc2[PAIR ? i : 0]);
     } else {
-      finish_one<T, 4>(a.e, m, (int)n, (int)a.N, acc[i]);
+      finish_one<float, 4>(a.e, m, (int)n, (int)a.N, acc[i]);
     }
   }
 }
@@ -176,7 +177,8 @@ __global__ void __launch_bounds__(256) split_sum_kernel(const float *partial, in
 
 // ------------------------------------------------------------------------------ derivative of the activation
 struct ActGradArgs {
-  const void *dy, *z;       // (M, N) and, for a pair, g and u of z at columns 0 and z_up
+  const void *dy;           // (M, N)
+  Saved z;                  // (M, N) or, for a pair, g and u at columns 0 and z_up
   long long ldy, ldz;
   int z_up;
   void *dz;                 // or null: only the sums
@@ -202,12 +204,12 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGradArgs a) {
     for (long long m = r0 + warp; m < r1; m += 8) {
       float dy[VEC], z[VEC], u[VEC], du[VEC];
       load_row<T, VEC>(static_cast<const T *>(a.dy) + m * a.ldy + n, VEC > 1, left, dy);
-      if (a.z != nullptr) load_row<T, VEC>(static_cast<const T *>(a.z) + m * a.ldz + n, VEC > 1, left, z);
-      if (PAIR) load_row<T, VEC>(static_cast<const T *>(a.z) + m * a.ldz + a.z_up + n, VEC > 1, left, u);
+      if (a.z.p != nullptr) load_saved<T, VEC>(a.z, m * a.ldz + n, VEC > 1, left, z);
+      if (PAIR) load_saved<T, VEC>(a.z, m * a.ldz + a.z_up + n, VEC > 1, left, u);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         float act = 0.f;
-        const float d = a.z != nullptr ? act_grad_of<T>(z[j], a.act, act) : 1.f;
+        const float d = a.z.p != nullptr ? act_grad_of<T>(z[j], a.act, act) : 1.f;
         if (PAIR) {
           du[j] = dy[j] * act;
           dy[j] = dy[j] * u[j] * d;
@@ -265,6 +267,25 @@ __global__ void __launch_bounds__(256) bias_sum_kernel(const float *partial, int
   if (db != nullptr) db[c < N ? c : c - N] = Cvt<T>::from_f(v);
 }
 
+// ------------------------------------------------------------------------------ rows on 16-byte boundaries
+// dst[r][c] = src[r][c] for c < cols, rows of dst `ldd` = cols rounded up to 8 apart; 8 elements a thread.  The tensor
+// cores' loads want rows that start on 16 bytes; operands with other strides (odd widths) go through this copy.
+__global__ void __launch_bounds__(256) copy_rows_kernel(const uint16_t *src, long long lds, uint16_t *dst, long long ldd,
+                                                        long long rows, long long cols) {
+  const long long packs = ldd / 8, i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * packs) return;
+  const long long r = i / packs, c = (i - r * packs) * 8;
+  uint16_t v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? src[r * lds + c + j] : 0;
+  uint4 o;
+  o.x = v[0] | (uint32_t)v[1] << 16;
+  o.y = v[2] | (uint32_t)v[3] << 16;
+  o.z = v[4] | (uint32_t)v[5] << 16;
+  o.w = v[6] | (uint32_t)v[7] << 16;
+  *reinterpret_cast<uint4 *>(dst + r * ldd + c) = o;
+}
+
 // ------------------------------------------------------------------------------ host
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -280,13 +301,23 @@ struct Scratch {
   }
 };
 
+// bytes of `rows` x `cols` kept pre-activations, and their two parts in a buffer
+int64_t saved_bytes(int64_t rows, int64_t cols, int dtype) {
+  return dtype == LA_F32 ? rows * cols * 4 : (rows * cols * 2 + 15) / 16 * 16 + rows * cols;
+}
+Saved saved_in(const void *p, int64_t rows, int64_t cols, int dtype) {
+  Saved s = {const_cast<void *>(p), nullptr};
+  if (p != nullptr && dtype != LA_F32)
+    s.low = static_cast<uint8_t *>(const_cast<void *>(p)) + (rows * cols * 2 + 15) / 16 * 16;
+  return s;
+}
+
 int epilogue_vec(const Epilogue &e, int dtype) {
   const int64_t per = 16 / (int64_t)dtype_size(dtype);
   return aligned16(e.bias[0]) && aligned16(e.bias[1]) && aligned16(e.residual) && aligned16(e.out) && aligned16(e.out2) &&
-         aligned16(e.save) && e.ldr % per == 0 && e.ldo % per == 0 && e.lds % per == 0 && e.save_up % per == 0;
+         aligned16(e.save.p) && e.ldr % per == 0 && e.ldo % per == 0 && e.lds % per == 0 && e.save_up % per == 0;
 }
 
-template <typename T>
 int simt_launch(const Product &p, int splits, float *partial, cudaStream_t st) {
   SimtArgs a = {};
   a.segments = p.segments;
@@ -304,8 +335,8 @@ int simt_launch(const Product &p, int splits, float *partial, cudaStream_t st) {
   a.partial = partial;
   const int64_t grid = mt * a.n_tiles * splits;
   if (grid > INT32_MAX) return LA_ERR_TOO_LARGE;
-  if (p.pair) simt_product_kernel<T, true><<<(unsigned)grid, 256, 0, st>>>(a);
-  else simt_product_kernel<T, false><<<(unsigned)grid, 256, 0, st>>>(a);
+  if (p.pair) simt_product_kernel<true><<<(unsigned)grid, 256, 0, st>>>(a);
+  else simt_product_kernel<false><<<(unsigned)grid, 256, 0, st>>>(a);
   return launch_status();
 }
 
@@ -318,30 +349,47 @@ int split_sum_launch(const Product &p, int splits, const float *partial, cudaStr
   return launch_status();
 }
 
+// The operand as the tensor cores can read it: itself, or its copy with rows on 16-byte boundaries.
+int readable(Operand &o, int64_t rows, int64_t cols, int dtype, Scratch &s, cudaStream_t st) {
+  if (dtype == LA_F32 || (aligned16(o.p) && o.ld % 8 == 0)) return LA_OK;
+  const int64_t ld = (cols + 7) / 8 * 8;
+  uint16_t *dst = static_cast<uint16_t *>(s.take(rows * ld * 2));
+  if (s.base != nullptr) {
+    const int64_t grid = (rows * (ld / 8) + 255) / 256;
+    if (grid > INT32_MAX) return LA_ERR_TOO_LARGE;
+    copy_rows_kernel<<<(unsigned)grid, 256, 0, st>>>(static_cast<const uint16_t *>(o.p), o.ld, dst, ld, rows, cols);
+    const int rc = launch_status();
+    if (rc != LA_OK) return rc;
+  }
+  o.p = dst;
+  o.ld = ld;
+  return LA_OK;
+}
+
 // One product with its epilogue.  With s.base null only the scratch is counted.
 int product(Product p, int dtype, Scratch s, int64_t &need, cudaStream_t st) {
-  const int64_t k = p.K[0] + (p.segments > 1 ? p.K[1] : 0);
-  const int64_t tiles = (p.M + kTile - 1) / kTile * ((p.N + kTile - 1) / kTile);
-  int64_t splits = 2 * (int64_t)sm_count() / tiles;  // two CTAs per SM at least, 128 terms a split at least
-  if (splits > k / 128) splits = k / 128;
-  if (splits > 16) splits = 16;
-  if (splits < 1) splits = 1;
+  GemmPlan plan = {0, 1};
+  if (dtype == LA_F32) {
+    const int64_t k = p.K[0] + (p.segments > 1 ? p.K[1] : 0);
+    const int64_t tiles = (p.M + kTile - 1) / kTile * ((p.N + kTile - 1) / kTile);
+    int64_t splits = 2 * (int64_t)sm_count() / tiles;  // two CTAs per SM at least, 128 terms a split at least
+    if (splits > k / 128) splits = k / 128;
+    if (splits > 16) splits = 16;
+    if (splits > 1) plan.splits = (int)splits;
+  } else {
+    plan = gemm_plan(p.M, p.N, p.K[0], p.segments > 1 ? p.K[1] : 0, p.pair != 0);
+  }
   float *partial = nullptr;
-  if (splits > 1) partial = static_cast<float *>(s.take(splits * (p.pair ? 2 : 1) * p.M * p.N * 4));
+  if (plan.splits > 1) partial = static_cast<float *>(s.take((int64_t)plan.splits * (p.pair ? 2 : 1) * p.M * p.N * 4));
   if (s.used > need) need = s.used;
   if (s.base == nullptr) return LA_OK;
   p.e.vec = epilogue_vec(p.e, dtype);
-  int rc = LA_ERR_UNSUPPORTED;
-  switch (dtype) {
-    case LA_F32: rc = simt_launch<float>(p, (int)splits, partial, st); break;
-    case LA_BF16: rc = simt_launch<__nv_bfloat16>(p, (int)splits, partial, st); break;
-    case LA_F16: rc = simt_launch<__half>(p, (int)splits, partial, st); break;
-  }
+  const int rc = dtype == LA_F32 ? simt_launch(p, plan.splits, partial, st) : gemm_launch(p, plan, partial, dtype, st);
   if (rc != LA_OK || partial == nullptr) return rc;
   switch (dtype) {
-    case LA_F32: return split_sum_launch<float>(p, (int)splits, partial, st);
-    case LA_BF16: return split_sum_launch<__nv_bfloat16>(p, (int)splits, partial, st);
-    case LA_F16: return split_sum_launch<__half>(p, (int)splits, partial, st);
+    case LA_F32: return split_sum_launch<float>(p, plan.splits, partial, st);
+    case LA_BF16: return split_sum_launch<__nv_bfloat16>(p, plan.splits, partial, st);
+    case LA_F16: return split_sum_launch<__half>(p, plan.splits, partial, st);
   }
   return LA_ERR_UNSUPPORTED;
 }
@@ -365,7 +413,7 @@ int act_grad_chunks(int64_t M, int64_t N, int dtype) {
 int act_grad(ActGradArgs a, bool pair, int chunks, void *db0, void *db1, int dtype, cudaStream_t st) {
   a.rows = (a.M + chunks - 1) / chunks;
   const int64_t per = 16 / (int64_t)dtype_size(dtype);
-  const bool vec = aligned16(a.dy) && aligned16(a.z) && aligned16(a.dz) && a.ldy % per == 0 && a.ldz % per == 0 &&
+  const bool vec = aligned16(a.dy) && aligned16(a.z.p) && aligned16(a.dz) && a.ldy % per == 0 && a.ldz % per == 0 &&
                    a.ldd % per == 0 && a.z_up % per == 0 && a.d_up % per == 0;
   switch (dtype) {
     case LA_F32: vec ? act_grad_launch<float, 4>(a, pair, chunks, st) : act_grad_launch<float, 1>(a, pair, chunks, st); break;
@@ -403,6 +451,10 @@ int forward(const FwdArgs &f, Scratch s, int64_t &need, cudaStream_t st) {
   p.a[0] = Operand{f.x, f.ldx, 0};
   p.b[0] = Operand{f.w[0], f.ldw[0], 0};
   p.b[1] = Operand{f.w[1], f.ldw[1], 0};
+  int rc = readable(p.a[0], f.M, f.K, f.dtype, s, st);
+  if (rc == LA_OK) rc = readable(p.b[0], f.N, f.K, f.dtype, s, st);
+  if (rc == LA_OK && f.pair) rc = readable(p.b[1], f.N, f.K, f.dtype, s, st);
+  if (rc != LA_OK) return rc;
   p.K[0] = f.K;
   p.segments = 1;
   p.pair = f.pair;
@@ -410,7 +462,7 @@ int forward(const FwdArgs &f, Scratch s, int64_t &need, cudaStream_t st) {
   p.e.bias[0] = f.bias[0]; p.e.bias[1] = f.bias[1];
   p.e.residual = f.residual; p.e.ldr = f.ldr;
   p.e.out = f.out; p.e.ldo = f.N; p.e.split = INT32_MAX; p.e.live = (int)f.M;
-  p.e.save = f.save; p.e.lds = f.pair ? 2 * f.N : f.N; p.e.save_up = f.pair ? (int)f.N : 0;
+  p.e.save = saved_in(f.save, f.M, f.pair ? 2 * f.N : f.N, f.dtype); p.e.lds = f.pair ? 2 * f.N : f.N; p.e.save_up = f.pair ? (int)f.N : 0;
   p.e.act = f.act;
   return product(p, f.dtype, s, need, st);
 }
@@ -437,14 +489,20 @@ int backward(const BwdArgs &f, Scratch s, int64_t &need, cudaStream_t st) {
   const bool own_dz = f.pair || f.act != kActNone;
   Operand dz = {f.dy, f.ldy, 0};
   if (own_dz && products) dz = Operand{s.take(f.M * (f.pair ? 2 * np : np) * es), f.pair ? 2 * np : np, 0};
+  Operand x = {f.x, f.ldx, 1}, w[2] = {{f.w[0], f.ldw[0], 1}, {f.w[1], f.ldw[1], 1}};
+  int rc = LA_OK;
+  if (!own_dz && products) rc = readable(dz, f.M, f.N, f.dtype, s, st);
+  if (rc == LA_OK && want_dw) rc = readable(x, f.M, f.K, f.dtype, s, st);
+  for (int i = 0; i < (f.pair ? 2 : 1) && f.dx != nullptr && rc == LA_OK; ++i)
+    rc = readable(w[i], f.N, f.K, f.dtype, s, st);
+  if (rc != LA_OK) return rc;
   const int chunks = act_grad_chunks(f.M, f.N, f.dtype);
   float *sums = want_db ? static_cast<float *>(s.take((int64_t)chunks * (f.pair ? 2 : 1) * f.N * 4)) : nullptr;
-  int rc;
   if (run && ((own_dz && products) || want_db)) {
     ActGradArgs a = {};
     a.dy = f.dy; a.ldy = f.ldy;
     if (own_dz) {
-      a.z = f.saved;
+      a.z = saved_in(f.saved, f.M, f.pair ? 2 * f.N : f.N, f.dtype);
       a.ldz = f.pair ? 2 * f.N : f.N;
       a.z_up = f.pair ? (int)f.N : 0;
     }
@@ -462,8 +520,8 @@ int backward(const BwdArgs &f, Scratch s, int64_t &need, cudaStream_t st) {
     Product p = {};
     p.a[0] = dz;
     p.a[1] = Operand{dz_up, dz.ld, 0};
-    p.b[0] = Operand{f.w[0], f.ldw[0], 1};
-    p.b[1] = Operand{f.w[1], f.ldw[1], 1};
+    p.b[0] = w[0];
+    p.b[1] = w[1];
     p.K[0] = f.N; p.K[1] = f.pair ? f.N : 0;
     p.segments = f.pair ? 2 : 1;
     p.M = f.M; p.N = f.K;
@@ -473,7 +531,7 @@ int backward(const BwdArgs &f, Scratch s, int64_t &need, cudaStream_t st) {
   if (want_dw) {
     Product p = {};
     p.a[0] = Operand{dz.p, dz.ld, 1};
-    p.b[0] = Operand{f.x, f.ldx, 1};
+    p.b[0] = x;
     p.K[0] = f.M;
     p.segments = 1;
     p.M = f.pair ? np + f.N : f.N;  // a pair: rows [0, N) are dWg, rows [np, np + N) dWu
@@ -551,6 +609,11 @@ using namespace la;
 using namespace la::lin;
 
 extern "C" {
+
+int64_t la_linear_saved_bytes(int64_t M, int64_t N, int dtype, int pair) {
+  const int rc = check_common(M, N, 1, dtype, kActNone);
+  return rc != LA_OK ? rc : saved_bytes(M, pair ? 2 * N : N, dtype);
+}
 
 int64_t la_linear_fwd_workspace_bytes(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *weight_up,
                                       int64_t ldw_up, int64_t M, int64_t N, int64_t K, int dtype) {

@@ -1,5 +1,6 @@
 // Pieces shared by the kernels of linear_fn and gated_linear_fn: what happens to a product before it is written
-// (bias, activation, product of the pair, residual), and the description of a product.
+// (bias, activation, product of the pair, residual), and the interface between the host plan (linear.cu) and the
+// matrix kernels (gemm_sm100.cu).
 #pragma once
 #include "common.cuh"
 
@@ -48,6 +49,13 @@ __device__ __forceinline__ float act_grad_of(float z, int kind, float &a) {
   return 1.f;
 }
 
+// Pre-activations kept for the backward: fp32 values, or (16-bit types) the upper 24 bits of fp32 values, 16 of them in
+// p and 8 in low.
+struct Saved {
+  void *p;
+  uint8_t *low;
+};
+
 // What becomes of a product.  One product: out = act(p + bias[0]) + residual, save = p + bias[0].  A pair (g, u):
 // out = act(g + bias[0]) * (u + bias[1]), save = g + bias[0] in columns [0, N) and u + bias[1] in [save_up, +N).
 // Rows: row m < split goes to out if m < live, else row m - split to out2 if that is < live (the two weight
@@ -59,11 +67,11 @@ struct Epilogue {
   void *out, *out2;
   long long ldo;
   int split, live;
-  void *save;
+  Saved save;
   long long lds;
   int save_up;
   int act;
-  int vec;  // every pointer 16-byte aligned, every row stride and save_up a multiple of 16 bytes
+  int vec;  // every pointer 16-byte aligned, every row stride and save_up a multiple of 16 bytes in the type of x
 };
 
 // W consecutive elements (W sizeof(T) = 8 or a multiple of 16 bytes) from / to p; `left` of them exist
@@ -119,6 +127,69 @@ __device__ __forceinline__ void store_row(T *p, bool vec, int left, const float 
   }
 }
 
+// W kept values at offset `off` (W a multiple of 8 where vec is set for a 16-bit type)
+template <typename T, int W>
+__device__ __forceinline__ void store_saved(const Saved &s, long long off, bool vec, int left, const float (&v)[W]) {
+  if constexpr (sizeof(T) == 4) {
+    store_row<float, W>(static_cast<float *>(s.p) + off, vec, left, v);
+  } else {
+    uint16_t *hi = static_cast<uint16_t *>(s.p) + off;
+    uint8_t *lo = s.low + off;
+    if constexpr (W % 8 == 0) {
+      if (vec && left >= W) {
+#pragma unroll
+        for (int i = 0; i < W; i += 8) {
+          uint32_t u[8], h[4], l[2];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) u[j] = __float_as_uint(v[i + j]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) h[j] = __byte_perm(u[2 * j], u[2 * j + 1], 0x7632);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            l[j] = __byte_perm(__byte_perm(u[4 * j], u[4 * j + 1], 0x0051), __byte_perm(u[4 * j + 2], u[4 * j + 3], 0x0051),
+                               0x5410);
+          *reinterpret_cast<uint4 *>(hi + i) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint2 *>(lo + i) = make_uint2(l[0], l[1]);
+        }
+        return;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+      if (j < left) {
+        hi[j] = (uint16_t)(__float_as_uint(v[j]) >> 16);
+        lo[j] = (uint8_t)(__float_as_uint(v[j]) >> 8);
+      }
+  }
+}
+template <typename T, int W>
+__device__ __forceinline__ void load_saved(const Saved &s, long long off, bool vec, int left, float (&v)[W]) {
+  if constexpr (sizeof(T) == 4) {
+    load_row<float, W>(static_cast<const float *>(s.p) + off, vec, left, v);
+  } else {
+    const uint16_t *hi = static_cast<const uint16_t *>(s.p) + off;
+    const uint8_t *lo = s.low + off;
+    if constexpr (W % 8 == 0) {
+      if (vec && left >= W) {
+#pragma unroll
+        for (int i = 0; i < W; i += 8) {
+          const uint4 h4 = *reinterpret_cast<const uint4 *>(hi + i);
+          const uint2 l2 = *reinterpret_cast<const uint2 *>(lo + i);
+          const uint32_t h[4] = {h4.x, h4.y, h4.z, h4.w}, l[2] = {l2.x, l2.y};
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {  // bytes: 0, low, high 16 bits
+            const uint32_t low = (l[j / 4] >> (8 * (j % 4))) & 0xffu;
+            v[i + j] = __uint_as_float((j % 2 ? h[j / 2] & 0xffff0000u : h[j / 2] << 16) | low << 8);
+          }
+        }
+        return;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[j] = j < left ? __uint_as_float((uint32_t)hi[j] << 16 | (uint32_t)lo[j] << 8) : 0.f;
+  }
+}
+
 template <typename T, int W>
 __device__ __forceinline__ void add_row(const void *p, long long off, bool vec, int left, float (&v)[W]) {
   if (p == nullptr) return;
@@ -142,7 +213,7 @@ __device__ __forceinline__ void finish_one(const Epilogue &e, long long m, int n
   T *row = out_row<T>(e, m);
   if (left <= 0 || row == nullptr) return;
   add_row<T, W>(e.bias[0], n, e.vec, left, p);
-  if (e.save != nullptr) store_row<T, W>(static_cast<T *>(e.save) + m * e.lds + n, e.vec, left, p);
+  if (e.save.p != nullptr) store_saved<T, W>(e.save, m * e.lds + n, e.vec, left, p);
   if (e.act != kActNone) {
 #pragma unroll
     for (int j = 0; j < W; ++j) p[j] = act_of<T>(p[j], e.act);
@@ -157,10 +228,9 @@ __device__ __forceinline__ void finish_pair(const Epilogue &e, long long m, int 
   if (left <= 0 || row == nullptr) return;
   add_row<T, W>(e.bias[0], n, e.vec, left, g);
   add_row<T, W>(e.bias[1], n, e.vec, left, u);
-  if (e.save != nullptr) {
-    T *s = static_cast<T *>(e.save) + m * e.lds + n;
-    store_row<T, W>(s, e.vec, left, g);
-    store_row<T, W>(s + e.save_up, e.vec, left, u);
+  if (e.save.p != nullptr) {
+    store_saved<T, W>(e.save, m * e.lds + n, e.vec, left, g);
+    store_saved<T, W>(e.save, m * e.lds + e.save_up + n, e.vec, left, u);
   }
 #pragma unroll
   for (int j = 0; j < W; ++j) g[j] = act_of<T>(g[j], e.act) * u[j];
@@ -184,6 +254,16 @@ struct Product {
   int64_t M, N;
   Epilogue e;
 };
+
+int sm_count();  // of the current device (148 where there is none); linear.cu
+
+// gemm_sm100.cu.  Number of splits of the contraction (partial sums in fp32, finished by another launch), its
+// workspace, and the launch.  16-bit operands with 16-byte aligned addresses and row strides.
+struct GemmPlan {
+  int bn, splits;
+};
+GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K0, int64_t K1, bool pair);
+int gemm_launch(const Product &p, const GemmPlan &plan, float *partial, int dtype, cudaStream_t st);
 
 }  // namespace lin
 }  // namespace la

@@ -4,8 +4,8 @@
     gated_linear_fn   h = act(x w_gate^T + b_gate) * (x w_up^T + b_up)
 
 x (..., K), weights (N, K) as torch.nn.Linear keeps them.  Products are accumulated in fp32 and rounded once, after
-bias, activation, product of the pair and residual.  Gradients for every tensor given.  Products run
-on the CUDA cores in fp32 for every type.  (The reference has the second projection of the pair as gate_linear,
+bias, activation, product of the pair and residual.  Gradients for every tensor given.  fp32 runs on the CUDA cores in
+fp32; bf16 and fp16 on the tensor cores.  (The reference has the second projection of the pair as gate_linear,
 xopes/ops/gate_linear, outside the attention path this library mirrors.)
 """
 from typing import Optional
@@ -46,9 +46,11 @@ class LinearFunction(torch.autograd.Function):
         n = w2.shape[0]
         b = None if bias is None else bias.contiguous()
         y = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=x.device)
-        z = torch.empty(m, n, dtype=x.dtype, device=x.device) if keep and act else None
+        code = _lib.dtype_code(x)
+        z = None
         if m:
-            code = _lib.dtype_code(x)
+            if keep and act:
+                z = _scratch(lib.la_linear_saved_bytes(m, n, code, 0), x.device)
             with _lib.device_of(x):
                 need = lib.la_linear_fwd_workspace_bytes(_lib.ptr(x2), ldx, _lib.ptr(w2), ldw, None, 0, m, n, k, code)
                 ws = _scratch(need, x.device)
@@ -97,9 +99,11 @@ class GatedLinearFunction(torch.autograd.Function):
         n = wg.shape[0]
         bg, bu = (None if b is None else b.contiguous() for b in (b_gate, b_up))
         h = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=x.device)
-        gu = torch.empty(m, 2 * n, dtype=x.dtype, device=x.device) if keep else None
+        code = _lib.dtype_code(x)
+        gu = None
         if m:
-            code = _lib.dtype_code(x)
+            if keep:
+                gu = _scratch(lib.la_linear_saved_bytes(m, n, code, 1), x.device)
             with _lib.device_of(x):
                 need = lib.la_linear_fwd_workspace_bytes(_lib.ptr(x2), ldx, _lib.ptr(wg), ldg, _lib.ptr(wu), ldu, m, n, k,
                                                          code)
@@ -177,7 +181,7 @@ def linear_fn(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor
 
     x (..., K), weight (N, K), bias (N), residual (..., N), all of one dtype; rows may be strided (slices need no copy).
     act: "none", "relu", "sigmoid", "silu" or "gelu" (the exact one, by erf).  The backward keeps x, the weight and,
-    with an activation, the pre-activation in x's dtype."""
+    with an activation, the pre-activation (24 bits a value, fp32: 32)."""
     keep = _check(x, [weight], [bias], residual, act)
     return LinearFunction.apply(x, weight, bias, residual, _ACTS[act], keep)
 
@@ -188,6 +192,6 @@ def gated_linear_fn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b
     and the product in one kernel.  The block's way down is linear_fn(h, w_down, residual=x).
 
     x (..., K), w_gate and w_up (N, K), biases (N), all of one dtype.  act as in linear_fn.  The backward keeps x, the
-    weights and both projections (2 N values a token) in x's dtype."""
+    weights and both projections (2 N values a token of 24 bits, fp32: 32)."""
     keep = _check(x, [w_gate, w_up], [b_gate, b_up], None, act)
     return GatedLinearFunction.apply(x, w_gate, w_up, b_gate, b_up, _ACTS[act], keep)
