@@ -33,14 +33,15 @@ constexpr int kStepK = 64;                 // contraction steps of a stage: 128 
 constexpr int kThreads = 384;
 constexpr int kEpiWarps = 8;
 constexpr uint32_t kABytes = 128 * 128;    // 128 rows of 128 bytes
+constexpr uint32_t kStrip = 32 * 256;      // an epilogue warp's 32 rows of 64 fp32 values
 constexpr int kGroup = 8;                  // rows of tiles walked together
 constexpr uint32_t kGroupBytes = 64 * 128; // 64 rows of an operand whose rows lie next to each other, 64 steps
 
 template <int BN> struct Cfg {
   static constexpr uint32_t kBBytes = BN / 2 * 128;
   static constexpr uint32_t kStage = kABytes + kBBytes;
-  static constexpr int kStages = BN == 256 ? 6 : 8;
-  static constexpr uint32_t kSmem = 1024 + kStages * kStage + 512;
+  static constexpr int kStages = BN == 256 ? 5 : 6;
+  static constexpr uint32_t kSmem = 1024 + kStages * kStage + kEpiWarps * kStrip + 512;
   static constexpr uint32_t kCols = 2 * BN;  // tensor memory: two accumulators
 };
 
@@ -115,12 +116,150 @@ __device__ __forceinline__ Unit unit_of(const GemmArgs &g, int u) {
   return x;
 }
 
+// An epilogue warp's strip: 32 rows of 64 fp32 values, 64 result columns or 32 of g and 32 of u.  Pieces of 16 bytes lie
+// where neither the writing lanes (8 rows, one piece) nor the reading lanes (kLanes lanes a row, 8 columns each) meet
+// in a bank.
+template <bool PAIR> struct Strip {
+  static constexpr int kCols = PAIR ? 32 : 64;
+  static constexpr int kLanes = kCols / 8;
+  static constexpr int kRowsAt = 32 / kLanes;  // rows the warp reads at a time
+  static __device__ __forceinline__ float4 *piece(float *strip, int row, int i) {
+    const int f = PAIR ? i : (i >> 1) | (i & 1) << 3;
+    return reinterpret_cast<float4 *>(strip) + row * 16 + (f ^ (row & 7));
+  }
+  // columns 8 cl .. 8 cl + 7 of a row; u: of the second product of a pair
+  static __device__ __forceinline__ void take(float *strip, int row, int cl, int u, float *v) {
+    const float4 x = *piece(strip, row, 8 * u + 2 * cl), y = *piece(strip, row, 8 * u + 2 * cl + 1);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+  }
+};
+
+template <typename T> __device__ __forceinline__ void unpack8(const uint4 &r, float *v) {
+  const T *h = reinterpret_cast<const T *>(&r);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = Cvt<T>::to_f(h[j]);
+}
+
+// where rows m0 .. m0 + 31 of the result go if they lie together, else null
+template <typename T> __device__ __forceinline__ T *out_rows(const Epilogue &e, long long m0) {
+  if (m0 + 32 <= e.split) return m0 + 32 <= e.live ? static_cast<T *>(e.out) + m0 * e.ldo : nullptr;
+  if (m0 < e.split) return nullptr;
+  return m0 - e.split + 32 <= e.live ? static_cast<T *>(e.out2) + (m0 - e.split) * e.ldo : nullptr;
+}
+
+// a strip that lies inside the matrix, everything on 16 bytes
+template <typename T, bool PAIR>
+__device__ __forceinline__ void inner_strip(const Epilogue &e, float *strip, T *out, long long m0, int n0, int lane) {
+  typedef Strip<PAIR> S;
+  constexpr int G = 4;
+  const int cl = lane % S::kLanes, rl = lane / S::kLanes, col = n0 + 8 * cl;
+  out += rl * e.ldo + col;
+  const long long ostep = S::kRowsAt * e.ldo;
+  float b0[8], b1[8];
+  if (e.bias[0] != nullptr) unpack8<T>(*reinterpret_cast<const uint4 *>(static_cast<const T *>(e.bias[0]) + col), b0);
+  if (PAIR && e.bias[1] != nullptr)
+    unpack8<T>(*reinterpret_cast<const uint4 *>(static_cast<const T *>(e.bias[1]) + col), b1);
+  const T *res = e.residual == nullptr ? nullptr : static_cast<const T *>(e.residual) + (m0 + rl) * e.ldr + col;
+  const long long rstep = S::kRowsAt * e.ldr;
+  long long kept = (m0 + rl) * e.lds + col;
+  const long long kstep = S::kRowsAt * e.lds;
+#pragma unroll 1
+  for (int i = 0; i < S::kLanes; i += G) {
+    uint4 r[G];
+    if (!PAIR && res != nullptr) {
+#pragma unroll
+      for (int k = 0; k < G; ++k) r[k] = *reinterpret_cast<const uint4 *>(res + k * rstep);
+      res += G * rstep;
+    }
+    float p[8 * G], q[8 * G];
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      S::take(strip, (i + k) * S::kRowsAt + rl, cl, 0, p + 8 * k);
+      if (PAIR) S::take(strip, (i + k) * S::kRowsAt + rl, cl, 1, q + 8 * k);
+    }
+    if (e.bias[0] != nullptr) {
+#pragma unroll
+      for (int k = 0; k < 8 * G; ++k) p[k] += b0[k & 7];
+    }
+    if (PAIR && e.bias[1] != nullptr) {
+#pragma unroll
+      for (int k = 0; k < 8 * G; ++k) q[k] += b1[k & 7];
+    }
+    if (e.save.p != nullptr) {
+#pragma unroll
+      for (int k = 0; k < G; ++k) {
+        store_saved<T, 8>(e.save, kept + k * kstep, true, 8, reinterpret_cast<const float (&)[8]>(p[8 * k]));
+        if (PAIR)
+          store_saved<T, 8>(e.save, kept + k * kstep + e.save_up, true, 8, reinterpret_cast<const float (&)[8]>(q[8 * k]));
+      }
+      kept += G * kstep;
+    }
+    activate<T, 8 * G>(p, e.act);
+    if (PAIR) {
+#pragma unroll
+      for (int k = 0; k < 8 * G; ++k) p[k] *= q[k];
+    } else if (e.residual != nullptr) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < G; ++k) {
+        unpack8<T>(r[k], v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[8 * k + j] += v[j];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < G; ++k)
+      store_row<T, 8>(out + k * ostep, true, 8, reinterpret_cast<const float (&)[8]>(p[8 * k]));
+    out += G * ostep;
+  }
+}
+
+// a strip at the edge, or tensors that are not on 16 bytes
+template <typename T, bool PAIR>
+__device__ __noinline__ void edge_strip(const Epilogue &e, float *strip, long long m0, int n0, int M, int N, int lane) {
+  typedef Strip<PAIR> S;
+  const int cl = lane % S::kLanes, rl = lane / S::kLanes, col = n0 + 8 * cl;
+#pragma unroll 1
+  for (int i = 0; i < S::kLanes; ++i) {
+    const int row = i * S::kRowsAt + rl;
+    float p[8], q[8];
+    S::take(strip, row, cl, 0, p);
+    if (PAIR) S::take(strip, row, cl, 1, q);
+    if (m0 + row >= M) continue;
+    if (PAIR) finish_pair<T, 8>(e, m0 + row, col, N, p, q);
+    else finish_one<T, 8>(e, m0 + row, col, N, p);
+  }
+}
+
+// a strip of one split's sums
+template <bool PAIR>
+__device__ __noinline__ void partial_strip(const GemmArgs &g, float *strip, int split, long long m0, int n0, int lane) {
+  typedef Strip<PAIR> S;
+  const int cl = lane % S::kLanes, rl = lane / S::kLanes, col = n0 + 8 * cl, left = g.N - col;
+  const bool vec = g.N % 4 == 0;
+  float *o = g.partial + ((long long)split * (PAIR ? 2 : 1) * g.M + m0 + rl) * g.N + col;
+#pragma unroll 4
+  for (int i = 0; i < S::kLanes; ++i, o += (long long)S::kRowsAt * g.N) {
+    const int row = i * S::kRowsAt + rl;
+    if (m0 + row >= g.M || left <= 0) break;
+    float p[8];
+    S::take(strip, row, cl, 0, p);
+    store_row<float, 8>(o, vec, left, p);
+    if (PAIR) {
+      S::take(strip, row, cl, 1, p);
+      store_row<float, 8>(o + (long long)g.M * g.N, vec, left, p);
+    }
+  }
+}
+
 template <typename T, bool A_MN, bool B_MN, int BN, bool PAIR>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ GemmArgs g) {
   typedef Cfg<BN> C;
   extern __shared__ uint8_t raw[];
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
-  const uint32_t bars = base + C::kStages * C::kStage;
+  const uint32_t strips = base + C::kStages * C::kStage;
+  const uint32_t bars = strips + kEpiWarps * kStrip;
   const uint32_t full = bars, empty = full + 8 * C::kStages, tfull = empty + 8 * C::kStages, tempty = tfull + 16;
   const uint32_t tmem_at = tempty + 16;
   volatile int *abort_flag = reinterpret_cast<volatile int *>(raw + (tmem_at + 4 - smem_u32(raw)));
@@ -233,41 +372,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue, in both CTAs
+    // A lane of tensor memory is a row, so a thread holds 64 columns of one row (32 of g and the same 32 of u).  Written
+    // from there, every store would touch 32 rows with 16 bytes each (the epilogue took 32,000 cycles a tile that way, 17 us);
+    // through a strip of shared memory of the warp's own 8 or 4 lanes share a row and a store touches 4 or 8 rows with
+    // 128 or 64 bytes.  With two warps per scheduler the latency of every instruction counts: four rows at a time, one
+    // branch per option for all four, pointers that only advance; strips at the matrix's edge go another way.
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     constexpr int kOut = PAIR ? BN / 2 : BN;  // result columns of a tile, half of them this warp's
+    float *strip = reinterpret_cast<float *>(raw + (strips - smem_u32(raw)) + (warp - 4) * kStrip);
     int n = 0;
     for (int u = first; u < units; u += stride, ++n) {
       const Unit x = unit_of<BN, PAIR>(g, u);
       const int buf = n & 1;
+      const long long m0 = (long long)x.m0 + rank * 128 + quarter * 32;
       if (!warp_wait(tfull + 8 * buf, (n >> 1) & 1, abort_flag, g.status, 305)) break;
       tc_fence_after();
-      const long long m = (long long)x.m0 + rank * 128 + quarter * 32 + lane;
-      const bool in = m < g.M;
       const uint32_t t0 = tmem + buf * BN + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
-      for (int c = half * (kOut / 2); c < (half + 1) * (kOut / 2); c += 16) {
-        __syncwarp();  // lanes past the last row skipped the stores
-        uint32_t r[16], r2[16];
-        tmem_ld16(t0 + c, r);
-        if (PAIR) tmem_ld16(t0 + kOut + c, r2);
-        tmem_wait_ld();
-        const int col = x.n0 + c;
-        if (!in || col >= g.N) continue;
-        float p[16], q[16];
+      for (int c = half * (kOut / 2); c < (half + 1) * (kOut / 2); c += Strip<PAIR>::kCols) {
+        const int n0 = x.n0 + c;
+        if (m0 >= g.M || n0 >= g.N) break;
+        {
+          uint32_t r[32], r2[32];
+          tmem_ld32(t0 + c, r);
+          tmem_ld32(t0 + c + (PAIR ? kOut : 32), r2);
+          tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          p[j] = __uint_as_float(r[j]);
-          q[j] = PAIR ? __uint_as_float(r2[j]) : 0.f;
+          for (int i = 0; i < 8; ++i) {
+            *Strip<PAIR>::piece(strip, lane, i) = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]),
+                                                              __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
+            *Strip<PAIR>::piece(strip, lane, i + 8) =
+                make_float4(__uint_as_float(r2[4 * i]), __uint_as_float(r2[4 * i + 1]), __uint_as_float(r2[4 * i + 2]),
+                            __uint_as_float(r2[4 * i + 3]));
+          }
         }
+        __syncwarp();
+        const bool inner = n0 + Strip<PAIR>::kCols <= g.N && m0 + 32 <= g.M;
         if (g.partial != nullptr) {
-          float *o = g.partial + ((long long)x.split * (PAIR ? 2 : 1) * g.M + m) * g.N + col;
-          store_row<float, 16>(o, g.N % 4 == 0, g.N - col, p);
-          if (PAIR) store_row<float, 16>(o + (long long)g.M * g.N, g.N % 4 == 0, g.N - col, q);
-        } else if (PAIR) {
-          finish_pair<T, 16>(g.e, m, col, g.N, p, q);
+          partial_strip<PAIR>(g, strip, x.split, m0, n0, lane);
         } else {
-          finish_one<T, 16>(g.e, m, col, g.N, p);
+          T *out = inner && g.e.vec ? out_rows<T>(g.e, m0) : nullptr;
+          if (out != nullptr) inner_strip<T, PAIR>(g.e, strip, out, m0, n0, lane);
+          else edge_strip<T, PAIR>(g.e, strip, m0, n0, g.M, g.N, lane);
         }
+        __syncwarp();
       }
       tc_fence_before();
       __syncwarp();

@@ -190,7 +190,8 @@ struct ActGradArgs {
   int act;
 };
 
-// CTA = 32 x VEC columns of one chunk of rows, a warp per row at a time.  One read of dy and z, one write of dz: HBM.
+// CTA = 32 x VEC columns of one chunk of rows, a warp per row at a time; the next row is loaded before the current one is
+// worked on.  One read of dy and of what was kept, one write of dz: HBM.
 template <typename T, int VEC, bool PAIR>
 __global__ void __launch_bounds__(256) act_grad_kernel(const ActGradArgs a) {
   __shared__ float part[PAIR ? 2 : 1][8][32 * VEC + 1];
@@ -198,32 +199,44 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGradArgs a) {
   const long long n = ((long long)blockIdx.x * 32 + lane) * VEC;
   const int left = a.N - n < VEC ? (int)(a.N - n) : VEC;
   const long long r0 = (long long)blockIdx.y * a.rows, r1 = r0 + a.rows < a.M ? r0 + a.rows : a.M;
+  const bool kept = a.z.p != nullptr;
   float s0[VEC] = {}, s1[VEC] = {};
   if (left > 0) {
-#pragma unroll 2
-    for (long long m = r0 + warp; m < r1; m += 8) {
-      float dy[VEC], z[VEC], u[VEC], du[VEC];
-      load_row<T, VEC>(static_cast<const T *>(a.dy) + m * a.ldy + n, VEC > 1, left, dy);
-      if (a.z.p != nullptr) load_saved<T, VEC>(a.z, m * a.ldz + n, VEC > 1, left, z);
-      if (PAIR) load_saved<T, VEC>(a.z, m * a.ldz + a.z_up + n, VEC > 1, left, u);
+    float dy[VEC], z[VEC], u[VEC], dy2[VEC], z2[VEC], u2[VEC];
+    auto fetch = [&](long long m, float (&d)[VEC], float (&p)[VEC], float (&q)[VEC]) {
+      load_row<T, VEC>(static_cast<const T *>(a.dy) + m * a.ldy + n, VEC > 1, left, d);
+      if (kept) load_saved<T, VEC>(a.z, m * a.ldz + n, VEC > 1, left, p);
+      if (PAIR) load_saved<T, VEC>(a.z, m * a.ldz + a.z_up + n, VEC > 1, left, q);
+    };
+    auto work = [&](long long m, float (&d)[VEC], float (&p)[VEC], float (&q)[VEC]) {
+      if (kept) {
+        float g[VEC];
+        activate_grad<T, VEC>(p, g, a.act);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float act = 0.f;
-        const float d = a.z.p != nullptr ? act_grad_of<T>(z[j], a.act, act) : 1.f;
-        if (PAIR) {
-          du[j] = dy[j] * act;
-          dy[j] = dy[j] * u[j] * d;
-          s1[j] += du[j];
-        } else {
-          dy[j] *= d;
+        for (int j = 0; j < VEC; ++j) {
+          if (PAIR) {
+            p[j] *= d[j];
+            d[j] *= q[j];
+            s1[j] += p[j];
+          }
+          d[j] *= g[j];
         }
-        s0[j] += dy[j];
       }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) s0[j] += d[j];
       if (a.dz != nullptr) {
         T *o = static_cast<T *>(a.dz) + m * a.ldd + n;
-        store_row<T, VEC>(o, VEC > 1, left, dy);
-        if (PAIR) store_row<T, VEC>(o + a.d_up, VEC > 1, left, du);
+        store_row<T, VEC>(o, VEC > 1, left, d);
+        if (PAIR) store_row<T, VEC>(o + a.d_up, VEC > 1, left, p);
       }
+    };
+    long long m = r0 + warp;
+    if (m < r1) fetch(m, dy, z, u);
+    for (; m < r1; m += 16) {
+      if (m + 8 < r1) fetch(m + 8, dy2, z2, u2);
+      work(m, dy, z, u);
+      if (m + 16 < r1) fetch(m + 16, dy, z, u);
+      if (m + 8 < r1) work(m + 8, dy2, z2, u2);
     }
   }
   if (a.partial == nullptr) return;  // uniform over the grid

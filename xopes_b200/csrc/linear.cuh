@@ -17,36 +17,57 @@ template <> __device__ __forceinline__ float inverse_of<float>(float x) { return
 // 1 / (1 + e^-z); the fast quotient returns 0 for divisors above 2^126, which is what the sigmoid is there
 template <typename T> __device__ __forceinline__ float sigmoid_of(float z) { return inverse_of<T>(1.f + exp_of<T>(-z)); }
 
-template <typename T>
-__device__ __forceinline__ float act_of(float z, int kind) {
-  switch (kind) {
-    case kActRelu: return z > 0.f || z != z ? z : 0.f;
-    case kActSigmoid: return sigmoid_of<T>(z);
-    case kActSilu: return z * sigmoid_of<T>(z);
-    case kActGelu: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+// z[j] = act(z[j]); the kind is the same for the whole launch, so the choice is a branch around a row's loop
+template <typename T, int W>
+__device__ __forceinline__ void activate(float (&z)[W], int kind) {
+  if (kind == kActRelu) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) z[j] = z[j] > 0.f || z[j] != z[j] ? z[j] : 0.f;
+  } else if (kind == kActSigmoid) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) z[j] = sigmoid_of<T>(z[j]);
+  } else if (kind == kActSilu) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) z[j] *= sigmoid_of<T>(z[j]);
+  } else if (kind == kActGelu) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) z[j] *= 0.5f + 0.5f * erff(z[j] * 0.70710678118654752f);
   }
-  return z;
 }
 
-// the activation and its derivative
-template <typename T>
-__device__ __forceinline__ float act_grad_of(float z, int kind, float &a) {
-  switch (kind) {
-    case kActRelu: a = z > 0.f || z != z ? z : 0.f; return z > 0.f ? 1.f : 0.f;
-    case kActSigmoid: a = sigmoid_of<T>(z); return a * (1.f - a);
-    case kActSilu: {
-      const float s = sigmoid_of<T>(z);
-      a = z * s;
-      return s * (1.f + z * (1.f - s));
+// z[j] = act(z[j]) and d[j] = act'(z[j])
+template <typename T, int W>
+__device__ __forceinline__ void activate_grad(float (&z)[W], float (&d)[W], int kind) {
+  if (kind == kActRelu) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      d[j] = z[j] > 0.f ? 1.f : 0.f;
+      z[j] = z[j] > 0.f || z[j] != z[j] ? z[j] : 0.f;
     }
-    case kActGelu: {
-      const float cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
-      a = z * cdf;
-      return cdf + z * 0.3989422804014327f * exp_of<T>(-0.5f * z * z);
+  } else if (kind == kActSigmoid) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      z[j] = sigmoid_of<T>(z[j]);
+      d[j] = z[j] * (1.f - z[j]);
     }
+  } else if (kind == kActSilu) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const float s = sigmoid_of<T>(z[j]);
+      d[j] = s * (1.f + z[j] * (1.f - s));
+      z[j] *= s;
+    }
+  } else if (kind == kActGelu) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const float cdf = 0.5f + 0.5f * erff(z[j] * 0.70710678118654752f);
+      d[j] = cdf + z[j] * 0.3989422804014327f * exp_of<T>(-0.5f * z[j] * z[j]);
+      z[j] *= cdf;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < W; ++j) d[j] = 1.f;
   }
-  a = z;
-  return 1.f;
 }
 
 // Pre-activations kept for the backward: fp32 values, or (16-bit types) the upper 24 bits of fp32 values, 16 of them in
@@ -214,10 +235,7 @@ __device__ __forceinline__ void finish_one(const Epilogue &e, long long m, int n
   if (left <= 0 || row == nullptr) return;
   add_row<T, W>(e.bias[0], n, e.vec, left, p);
   if (e.save.p != nullptr) store_saved<T, W>(e.save, m * e.lds + n, e.vec, left, p);
-  if (e.act != kActNone) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) p[j] = act_of<T>(p[j], e.act);
-  }
+  activate<T, W>(p, e.act);
   add_row<T, W>(e.residual, m * e.ldr + n, e.vec, left, p);
   store_row<T, W>(row + n, e.vec, left, p);
 }
@@ -232,8 +250,9 @@ __device__ __forceinline__ void finish_pair(const Epilogue &e, long long m, int 
     store_saved<T, W>(e.save, m * e.lds + n, e.vec, left, g);
     store_saved<T, W>(e.save, m * e.lds + e.save_up + n, e.vec, left, u);
   }
+  activate<T, W>(g, e.act);
 #pragma unroll
-  for (int j = 0; j < W; ++j) g[j] = act_of<T>(g[j], e.act) * u[j];
+  for (int j = 0; j < W; ++j) g[j] *= u[j];
   store_row<T, W>(row + n, e.vec, left, g);
 }
 
