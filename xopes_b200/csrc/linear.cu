@@ -190,53 +190,97 @@ struct ActGradArgs {
   int act;
 };
 
-// CTA = 32 x VEC columns of one chunk of rows, a warp per row at a time; the next row is loaded before the current one is
+// VEC values of a row, and VEC kept ones, as they come from memory: nothing touches them until they are needed, so that
+// loads issued ahead stay in flight
+template <typename T, int VEC> struct RawRow {
+  uint4 r;
+  __device__ __forceinline__ void load(const T *p) { r = *reinterpret_cast<const uint4 *>(p); }
+  __device__ __forceinline__ void get(float (&v)[VEC]) const {
+    const T *h = reinterpret_cast<const T *>(&r);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = Cvt<T>::to_f(h[j]);
+  }
+};
+template <typename T> struct RawRow<T, 1> {
+  T r;
+  __device__ __forceinline__ void load(const T *p) { r = *p; }
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = Cvt<T>::to_f(r); }
+};
+template <typename T, int VEC> struct RawKept {
+  uint4 h;
+  uint2 l;
+  __device__ __forceinline__ void load(const Saved &s, long long off) {
+    h = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(s.p) + off);
+    l = *reinterpret_cast<const uint2 *>(s.low + off);
+  }
+  __device__ __forceinline__ void get(float (&v)[VEC]) const { kept_values(h, l, v); }
+};
+template <> struct RawKept<float, 4> {
+  RawRow<float, 4> r;
+  __device__ __forceinline__ void load(const Saved &s, long long off) { r.load(static_cast<const float *>(s.p) + off); }
+  __device__ __forceinline__ void get(float (&v)[4]) const { r.get(v); }
+};
+template <typename T> struct RawKept<T, 1> {
+  float r;
+  __device__ __forceinline__ void load(const Saved &s, long long off) {
+    float v[1];
+    load_saved<T, 1>(s, off, false, 1, v);
+    r = v[0];
+  }
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = r; }
+};
+
+// CTA = 32 x VEC columns of one chunk of rows, a warp per row at a time, two rows in flight ahead of the two that are
 // worked on.  One read of dy and of what was kept, one write of dz: HBM.
 template <typename T, int VEC, bool PAIR>
-__global__ void __launch_bounds__(256) act_grad_kernel(const ActGradArgs a) {
+__global__ void __launch_bounds__(256, PAIR ? 2 : 3) act_grad_kernel(const ActGradArgs a) {
   __shared__ float part[PAIR ? 2 : 1][8][32 * VEC + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long n = ((long long)blockIdx.x * 32 + lane) * VEC;
-  const int left = a.N - n < VEC ? (int)(a.N - n) : VEC;
   const long long r0 = (long long)blockIdx.y * a.rows, r1 = r0 + a.rows < a.M ? r0 + a.rows : a.M;
   const bool kept = a.z.p != nullptr;
   float s0[VEC] = {}, s1[VEC] = {};
-  if (left > 0) {
-    float dy[VEC], z[VEC], u[VEC], dy2[VEC], z2[VEC], u2[VEC];
-    auto fetch = [&](long long m, float (&d)[VEC], float (&p)[VEC], float (&q)[VEC]) {
-      load_row<T, VEC>(static_cast<const T *>(a.dy) + m * a.ldy + n, VEC > 1, left, d);
-      if (kept) load_saved<T, VEC>(a.z, m * a.ldz + n, VEC > 1, left, p);
-      if (PAIR) load_saved<T, VEC>(a.z, m * a.ldz + a.z_up + n, VEC > 1, left, q);
-    };
-    auto work = [&](long long m, float (&d)[VEC], float (&p)[VEC], float (&q)[VEC]) {
-      if (kept) {
-        float g[VEC];
-        activate_grad<T, VEC>(p, g, a.act);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          if (PAIR) {
-            p[j] *= d[j];
-            d[j] *= q[j];
-            s1[j] += p[j];
-          }
-          d[j] *= g[j];
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) s0[j] += d[j];
-      if (a.dz != nullptr) {
-        T *o = static_cast<T *>(a.dz) + m * a.ldd + n;
-        store_row<T, VEC>(o, VEC > 1, left, d);
-        if (PAIR) store_row<T, VEC>(o + a.d_up, VEC > 1, left, p);
-      }
+  if (n < a.N) {  // N is a multiple of VEC
+    RawRow<T, VEC> dy[2];
+    RawKept<T, VEC> z[2], u[2];
+    auto fetch = [&](long long m, int i) {
+      dy[i].load(static_cast<const T *>(a.dy) + m * a.ldy + n);
+      if (kept) z[i].load(a.z, m * a.ldz + n);
+      if (PAIR) u[i].load(a.z, m * a.ldz + a.z_up + n);
     };
     long long m = r0 + warp;
-    if (m < r1) fetch(m, dy, z, u);
+    if (m < r1) fetch(m, 0);
+    if (m + 8 < r1) fetch(m + 8, 1);
     for (; m < r1; m += 16) {
-      if (m + 8 < r1) fetch(m + 8, dy2, z2, u2);
-      work(m, dy, z, u);
-      if (m + 16 < r1) fetch(m + 16, dy, z, u);
-      if (m + 8 < r1) work(m + 8, dy2, z2, u2);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const long long mi = m + 8 * i;
+        if (mi >= r1) break;
+        float d[VEC], p[VEC], q[VEC], g[VEC];
+        dy[i].get(d);
+        if (kept) z[i].get(p);
+        if (PAIR) u[i].get(q);
+        if (mi + 16 < r1) fetch(mi + 16, i);
+        if (kept) {
+          activate_grad<T, VEC>(p, g, a.act);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            if (PAIR) {
+              p[j] *= d[j];
+              d[j] *= q[j];
+              s1[j] += p[j];
+            }
+            d[j] *= g[j];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s0[j] += d[j];
+        if (a.dz != nullptr) {
+          T *o = static_cast<T *>(a.dz) + mi * a.ldd + n;
+          store_row<T, VEC>(o, VEC > 1, VEC, d);
+          if (PAIR) store_row<T, VEC>(o + a.d_up, VEC > 1, VEC, p);
+        }
+      }
     }
   }
   if (a.partial == nullptr) return;  // uniform over the grid
@@ -414,10 +458,10 @@ void act_grad_launch(const ActGradArgs &a, bool pair, int chunks, cudaStream_t s
   else act_grad_kernel<T, VEC, false><<<grid, 256, 0, st>>>(a);
 }
 
-// chunks of rows of act_grad_kernel: four CTAs per SM, at least 8 rows (one per warp) a chunk
-int act_grad_chunks(int64_t M, int64_t N, int dtype) {
+// chunks of rows of act_grad_kernel: one wave of the CTAs that fit, at least 8 rows (one per warp) a chunk
+int act_grad_chunks(int64_t M, int64_t N, int dtype, bool pair) {
   const int64_t cols = 32 * (16 / (int64_t)dtype_size(dtype));
-  int64_t chunks = 8 * (int64_t)sm_count() / ((N + cols - 1) / cols);
+  int64_t chunks = (pair ? 2 : 3) * (int64_t)sm_count() / ((N + cols - 1) / cols);
   if (chunks > (M + 7) / 8) chunks = (M + 7) / 8;
   if (chunks > 4096) chunks = 4096;
   return chunks < 1 ? 1 : (int)chunks;
@@ -427,7 +471,7 @@ int act_grad(ActGradArgs a, bool pair, int chunks, void *db0, void *db1, int dty
   a.rows = (a.M + chunks - 1) / chunks;
   const int64_t per = 16 / (int64_t)dtype_size(dtype);
   const bool vec = aligned16(a.dy) && aligned16(a.z.p) && aligned16(a.dz) && a.ldy % per == 0 && a.ldz % per == 0 &&
-                   a.ldd % per == 0 && a.z_up % per == 0 && a.d_up % per == 0;
+                   a.ldd % per == 0 && a.z_up % per == 0 && a.d_up % per == 0 && a.N % per == 0;
   switch (dtype) {
     case LA_F32: vec ? act_grad_launch<float, 4>(a, pair, chunks, st) : act_grad_launch<float, 1>(a, pair, chunks, st); break;
     case LA_BF16:
@@ -509,7 +553,7 @@ int backward(const BwdArgs &f, Scratch s, int64_t &need, cudaStream_t st) {
   for (int i = 0; i < (f.pair ? 2 : 1) && f.dx != nullptr && rc == LA_OK; ++i)
     rc = readable(w[i], f.N, f.K, f.dtype, s, st);
   if (rc != LA_OK) return rc;
-  const int chunks = act_grad_chunks(f.M, f.N, f.dtype);
+  const int chunks = act_grad_chunks(f.M, f.N, f.dtype, f.pair != 0);
   float *sums = want_db ? static_cast<float *>(s.take((int64_t)chunks * (f.pair ? 2 : 1) * f.N * 4)) : nullptr;
   if (run && ((own_dz && products) || want_db)) {
     ActGradArgs a = {};

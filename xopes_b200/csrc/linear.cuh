@@ -17,6 +17,21 @@ template <> __device__ __forceinline__ float inverse_of<float>(float x) { return
 // 1 / (1 + e^-z); the fast quotient returns 0 for divisors above 2^126, which is what the sigmoid is there
 template <typename T> __device__ __forceinline__ float sigmoid_of(float z) { return inverse_of<T>(1.f + exp_of<T>(-z)); }
 
+// Phi(z), the normal distribution's integral, with e = e^(-z^2 / 2).  fp32: by erf.  Where the result is rounded to 16
+// bits: Abramowitz and Stegun 7.1.26, 1 - (a1 t + .. + a5 t^5) e with t = 1 / (1 + p |z| / sqrt 2), absolute error
+// 1.5e-7, which shares its exponential with the density (erff took 2/3 of the derivative pass's instructions).
+template <typename T> __device__ __forceinline__ float normal_cdf(float z, float &e) {
+  e = exp_of<T>(-0.5f * z * z);
+  const float t = __fdividef(1.f, fmaf(0.23164189f, fabsf(z), 1.f));
+  const float q = t * e * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f),
+                               0.127414796f);
+  return z < 0.f ? q : 1.f - q;
+}
+template <> __device__ __forceinline__ float normal_cdf<float>(float z, float &e) {
+  e = expf(-0.5f * z * z);
+  return 0.5f + 0.5f * erff(z * 0.70710678118654752f);
+}
+
 // z[j] = act(z[j]); the kind is the same for the whole launch, so the choice is a branch around a row's loop
 template <typename T, int W>
 __device__ __forceinline__ void activate(float (&z)[W], int kind) {
@@ -31,7 +46,10 @@ __device__ __forceinline__ void activate(float (&z)[W], int kind) {
     for (int j = 0; j < W; ++j) z[j] *= sigmoid_of<T>(z[j]);
   } else if (kind == kActGelu) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) z[j] *= 0.5f + 0.5f * erff(z[j] * 0.70710678118654752f);
+    for (int j = 0; j < W; ++j) {
+      float e;
+      z[j] *= normal_cdf<T>(z[j], e);
+    }
   }
 }
 
@@ -60,8 +78,9 @@ __device__ __forceinline__ void activate_grad(float (&z)[W], float (&d)[W], int 
   } else if (kind == kActGelu) {
 #pragma unroll
     for (int j = 0; j < W; ++j) {
-      const float cdf = 0.5f + 0.5f * erff(z[j] * 0.70710678118654752f);
-      d[j] = cdf + z[j] * 0.3989422804014327f * exp_of<T>(-0.5f * z[j] * z[j]);
+      float e;
+      const float cdf = normal_cdf<T>(z[j], e);
+      d[j] = cdf + z[j] * 0.3989422804014327f * e;
       z[j] *= cdf;
     }
   } else {
@@ -183,6 +202,14 @@ __device__ __forceinline__ void store_saved(const Saved &s, long long off, bool 
       }
   }
 }
+// Eight kept values of 24 bits out of their upper 16 and lower 8.  The 8 bits that were cut off are filled with a copy of
+// the lower 8: one instruction a value, and the errors of the cut are centred.
+__device__ __forceinline__ void kept_values(const uint4 &h4, const uint2 &l2, float *v) {
+  const uint32_t h[4] = {h4.x, h4.y, h4.z, h4.w}, l[2] = {l2.x, l2.y};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    v[j] = __uint_as_float(__byte_perm(l[j / 4], h[j / 2], (j % 4) * 0x11 + (j % 2 ? 0x7600 : 0x5400)));
+}
 template <typename T, int W>
 __device__ __forceinline__ void load_saved(const Saved &s, long long off, bool vec, int left, float (&v)[W]) {
   if constexpr (sizeof(T) == 4) {
@@ -193,21 +220,13 @@ __device__ __forceinline__ void load_saved(const Saved &s, long long off, bool v
     if constexpr (W % 8 == 0) {
       if (vec && left >= W) {
 #pragma unroll
-        for (int i = 0; i < W; i += 8) {
-          const uint4 h4 = *reinterpret_cast<const uint4 *>(hi + i);
-          const uint2 l2 = *reinterpret_cast<const uint2 *>(lo + i);
-          const uint32_t h[4] = {h4.x, h4.y, h4.z, h4.w}, l[2] = {l2.x, l2.y};
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {  // bytes: 0, low, high 16 bits
-            const uint32_t low = (l[j / 4] >> (8 * (j % 4))) & 0xffu;
-            v[i + j] = __uint_as_float((j % 2 ? h[j / 2] & 0xffff0000u : h[j / 2] << 16) | low << 8);
-          }
-        }
+        for (int i = 0; i < W; i += 8)
+          kept_values(*reinterpret_cast<const uint4 *>(hi + i), *reinterpret_cast<const uint2 *>(lo + i), v + i);
         return;
       }
     }
 #pragma unroll
-    for (int j = 0; j < W; ++j) v[j] = j < left ? __uint_as_float((uint32_t)hi[j] << 16 | (uint32_t)lo[j] << 8) : 0.f;
+    for (int j = 0; j < W; ++j) v[j] = j < left ? __uint_as_float((uint32_t)hi[j] << 16 | (uint32_t)lo[j] * 0x101u) : 0.f;
   }
 }
 
