@@ -118,6 +118,20 @@ def test_tokens_and_heads(b, n, h, hk):
     check(b, n, h, hk, 64, 64, torch.float32, interleaved=True)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,n,h,hk,d,r", [(3, 501, 16, 16, 128, 128), (1, 1777, 21, 9, 96, 64), (2, 2049, 13, 2, 64, 64),
+                                          (1, 700, 40, 8, 256, 256), (2, 300, 17, 17, 512, 512), (1, 5000, 32, 32, 32, 16),
+                                          (1, 60000, 1, 1, 64, 64)])
+def test_large_calls(b, n, h, hk, d, r, dtype):
+    check(b, n, h, hk, d, r, dtype, interleaved=bool(n % 2))
+
+    def cut(t):  # heads cut from a projection: other strides for tokens than for heads
+        buf = torch.zeros(b, n, t.shape[2] + 2, d, dtype=t.dtype)
+        buf[:, :, 2:] = t
+        return buf.cuda()[:, :, 2:].detach()
+    check(b, n, h, hk, d, r, dtype, interleaved=not n % 2, make=cut, seed=1)
+
+
 @pytest.mark.parametrize("where", ["packed", "transposed", "offset4", "offset1", "expanded"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_strides_and_alignment(where, dtype):

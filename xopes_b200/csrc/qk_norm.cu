@@ -20,7 +20,14 @@
 // becomes fp32: exact to 2^-24 turns for positions up to 2^28, where fp32 products are off by whole turns.
 // The weight gradient stays in registers over all rows of a lane, and leaves as one partial row per CTA,
 // which a second kernel adds in a fixed order.
+//
+// Two kernels.  qk_norm_stream_kernel, for large calls whose heads lie next to each other: every warp keeps a ring of
+// slots in shared memory full by bulk copies of several heads of a token, so that the bytes in flight do not depend on
+// registers.  qk_norm_kernel, for small calls, other strides and few heads: loads straight into registers, one step ahead.
+// 8 x 8192 tokens of 32 + 32 heads of 128 (bf16), forward / backward: 375-390 / 535 us by the first (2.15 / 3.22 GB, 328 /
+// 492 us at the measured copy bandwidth), 531 / 932 by the second.
 #include "common.cuh"
+#include "sm100_ptx.cuh"
 
 namespace la {
 namespace {
@@ -28,6 +35,7 @@ namespace {
 constexpr int kMaxD = 512;
 constexpr int kThreads = 128, kWarps = kThreads / 32;
 constexpr int kMaxCtas = 2048;  // partial rows of the weight gradients
+constexpr long long kStreamFrom = 1 << 20;  // elements of a tensor (launch_both)
 
 struct QkArgs {
   const void *x[2];           // q, k
@@ -96,10 +104,153 @@ __device__ __forceinline__ long long position_of(const QkArgs &a, long long t) {
   return n + a.offset;
 }
 
+// The features of a lane and its share of the weights and their gradients.
 // INTER: interleaved pairs.  VEC > 1: pack p of lane l (p LPR + l = j) is the low features [j VEC, +VEC) of the
 // first half of the rotated (or of the passing) features and the matching high ones; with INTER the "low" and
 // "high" packs are simply the first and second half of the row, and pairs are neighbours inside a pack.
 // VEC == 1: any D, R and alignment, INTER read from `inter`.
+template <typename T, bool INTER, int VEC, int LPR, int NP> struct Lane {
+  static constexpr int N = VEC * NP;
+  int f_lo[NP], f_hi[NP];
+  bool on_lo[NP], on_hi[NP];
+  float w_lo[N], w_hi[N];  // c w
+
+  __device__ __forceinline__ void init(const QkArgs &a, int which, int inter, int gl) {
+    const int D = a.D, half = a.R >> 1, pairs = (D + 1) >> 1;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int j = (p * LPR + gl) * VEC;
+      on_lo[p] = j < pairs;
+      if (VEC == 1 ? inter != 0 : INTER) {
+        f_lo[p] = VEC == 1 ? 2 * j : j;
+        f_hi[p] = VEC == 1 ? 2 * j + 1 : j + (D >> 1);
+      } else if (j < half) {
+        f_lo[p] = j;
+        f_hi[p] = j + half;
+      } else {
+        f_lo[p] = j + half;
+        f_hi[p] = j + half + ((D - a.R + 1) >> 1);
+      }
+      on_hi[p] = on_lo[p] && f_hi[p] < D;
+    }
+    const void *wp = a.w[which];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int p = i / VEC, j = i % VEC;
+      w_lo[i] = w_hi[i] = a.c;
+      if (wp != nullptr) {
+        if (on_lo[p])
+          w_lo[i] *= a.w16 ? Cvt<T>::to_f(static_cast<const T *>(wp)[f_lo[p] + j]) : static_cast<const float *>(wp)[f_lo[p] + j];
+        if (on_hi[p])
+          w_hi[i] *= a.w16 ? Cvt<T>::to_f(static_cast<const T *>(wp)[f_hi[p] + j]) : static_cast<const float *>(wp)[f_hi[p] + j];
+      }
+    }
+  }
+  // the lane's angles out of a token's (SIGN: of the rotation)
+  __device__ __forceinline__ void angles(const float *c, const float *s, int half, int gl, float sign, float (&cs)[N],
+                                         float (&sn)[N]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int p = i / VEC, j = i % VEC;
+      int pr = (p * LPR + gl) * VEC + j;  // the lane's i-th pair
+      if (INTER && VEC > 1)               // first half of the values: pairs of the low pack, then of the high pack
+        pr = ((j < VEC / 2 ? f_lo[p] : f_hi[p]) >> 1) + j % (VEC / 2 > 0 ? VEC / 2 : 1);
+      const bool rot = pr < half;
+      cs[i] = rot ? c[pr] : 1.f;
+      sn[i] = rot ? sign * s[pr] : 0.f;
+    }
+  }
+  static __device__ __forceinline__ void rotate(float *lo, float *hi, const float (&cs)[N], const float (&sn)[N]) {
+    if (INTER && VEC > 1) {
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+          const int e = p * VEC + 2 * j, cl = p * VEC + j, ch = cl + VEC / 2;
+          const float a0 = lo[e], a1 = lo[e + 1], b0 = hi[e], b1 = hi[e + 1];
+          lo[e] = a0 * cs[cl] - a1 * sn[cl];
+          lo[e + 1] = a1 * cs[cl] + a0 * sn[cl];
+          hi[e] = b0 * cs[ch] - b1 * sn[ch];
+          hi[e + 1] = b1 * cs[ch] + b0 * sn[ch];
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float u = lo[i], v = hi[i];
+        lo[i] = u * cs[i] - v * sn[i];
+        hi[i] = v * cs[i] + u * sn[i];
+      }
+    }
+  }
+  // (xl, xh): a row in, its output out
+  __device__ __forceinline__ void forward(float (&xl)[N], float (&xh)[N], const float (&cs)[N], const float (&sn)[N],
+                                          float eps) const {
+    float s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) s2 += xl[i] * xl[i] + xh[i] * xh[i];
+    const float rs = rsqrtf(lane_sum<LPR>(s2) + eps);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      xl[i] = xl[i] * rs * w_lo[i];
+      xh[i] = xh[i] * rs * w_hi[i];
+    }
+    rotate(xl, xh, cs, sn);
+  }
+  // (xl, xh): a row in, its gradient out; (dl, dh): the output's gradient; sn negative: the rotation back
+  __device__ __forceinline__ void backward(float (&xl)[N], float (&xh)[N], float (&dl)[N], float (&dh)[N],
+                                           const float (&cs)[N], const float (&sn)[N], float eps, float (&dw_lo)[N],
+                                           float (&dw_hi)[N]) const {
+    rotate(dl, dh, cs, sn);
+    float s2 = 0.f, dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      s2 += xl[i] * xl[i] + xh[i] * xh[i];
+      dot += dl[i] * w_lo[i] * xl[i] + dh[i] * w_hi[i] * xh[i];
+    }
+    const float rs = rsqrtf(lane_sum<LPR>(s2) + eps);
+    dot = lane_sum<LPR>(dot) * rs;  // sum of g xh
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float nl = xl[i] * rs, nh = xh[i] * rs;
+      dw_lo[i] += nl * dl[i];
+      dw_hi[i] += nh * dh[i];
+      xl[i] = (dl[i] * w_lo[i] - nl * dot) * rs;
+      xh[i] = (dh[i] * w_hi[i] - nh * dot) * rs;
+    }
+  }
+  // the CTA's partial weight gradient: sums over the warps' rows
+  __device__ __forceinline__ void leave(float (&dw_lo)[N], float (&dw_hi)[N], float (*part)[2 * LPR * N], float *out,
+                                        const QkArgs &a, int warp, int sub) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+#pragma unroll
+      for (int o = LPR; o < 32; o <<= 1) {
+        dw_lo[i] += __shfl_xor_sync(0xffffffffu, dw_lo[i], o);
+        dw_hi[i] += __shfl_xor_sync(0xffffffffu, dw_hi[i], o);
+      }
+      const int p = i / VEC, j = i % VEC;
+      if (sub == 0) {
+        if (on_lo[p]) part[warp][f_lo[p] + j] = dw_lo[i];
+        if (on_hi[p]) part[warp][f_hi[p] + j] = dw_hi[i];
+      }
+    }
+    __syncthreads();
+    for (int f = threadIdx.x; f < a.D; f += kThreads) {
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) s += part[k][f];
+      out[f] = s * a.c;
+    }
+  }
+};
+
+// angle of a position as cosine and sine
+__device__ __forceinline__ void angle_of(long long position, double freq, float &c, float &s) {
+  double turns = (double)position * freq;
+  turns -= rint(turns);
+  sincospif(2.f * (float)turns, &s, &c);
+}
+
 template <typename T, bool BWD, bool INTER, int VEC, int LPR, int NP>
 __global__ void __launch_bounds__(kThreads) qk_norm_kernel(const __grid_constant__ QkArgs a, const int inter) {
   typedef Pack<T, VEC> P;
@@ -113,43 +264,11 @@ __global__ void __launch_bounds__(kThreads) qk_norm_kernel(const __grid_constant
   const int which = blockIdx.x >= (unsigned)a.ctas[0];
   const int cta = which ? blockIdx.x - a.ctas[0] : blockIdx.x;
   const int H = a.heads[which], D = a.D, half = a.R >> 1;
-  const int pairs = (D + 1) >> 1;
   for (int i = threadIdx.x; i < half; i += kThreads) s_freq[i] = a.freq[i];
   __syncthreads();
-
-  // features of the lane's packs (one low, one high), and which exist
-  int f_lo[NP], f_hi[NP];
-  bool on_lo[NP], on_hi[NP];
-#pragma unroll
-  for (int p = 0; p < NP; ++p) {
-    const int j = (p * LPR + gl) * VEC;
-    on_lo[p] = j < pairs;
-    if (VEC == 1 ? inter != 0 : INTER) {
-      f_lo[p] = VEC == 1 ? 2 * j : j;
-      f_hi[p] = VEC == 1 ? 2 * j + 1 : j + (D >> 1);
-    } else if (j < half) {
-      f_lo[p] = j;
-      f_hi[p] = j + half;
-    } else {
-      f_lo[p] = j + half;
-      f_hi[p] = j + half + ((D - a.R + 1) >> 1);
-    }
-    on_hi[p] = on_lo[p] && f_hi[p] < D;
-  }
-  float w_lo[N], w_hi[N], dw_lo[N], dw_hi[N];
-  const void *wp = a.w[which];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int p = i / VEC, j = i % VEC;
-    w_lo[i] = w_hi[i] = a.c;
-    if (wp != nullptr) {
-      if (on_lo[p])
-        w_lo[i] *= a.w16 ? Cvt<T>::to_f(static_cast<const T *>(wp)[f_lo[p] + j]) : static_cast<const float *>(wp)[f_lo[p] + j];
-      if (on_hi[p])
-        w_hi[i] *= a.w16 ? Cvt<T>::to_f(static_cast<const T *>(wp)[f_hi[p] + j]) : static_cast<const float *>(wp)[f_hi[p] + j];
-    }
-    dw_lo[i] = dw_hi[i] = 0.f;
-  }
+  Lane<T, INTER, VEC, LPR, NP> ln;
+  ln.init(a, which, inter, gl);
+  float dw_lo[N] = {}, dw_hi[N] = {};
   const T *xp = static_cast<const T *>(a.x[which]);
   const T *dp = BWD ? static_cast<const T *>(a.d_out[which]) : nullptr;
   T *op = static_cast<T *>(a.out[which]);
@@ -177,12 +296,12 @@ __global__ void __launch_bounds__(kThreads) qk_norm_kernel(const __grid_constant
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
         const T *x = xrow + hc * a.sh[which];
-        r_lo[p] = on_lo[p] ? *reinterpret_cast<const R *>(x + f_lo[p]) : zero;
-        r_hi[p] = on_hi[p] ? *reinterpret_cast<const R *>(x + f_hi[p]) : zero;
+        r_lo[p] = ln.on_lo[p] ? *reinterpret_cast<const R *>(x + ln.f_lo[p]) : zero;
+        r_hi[p] = ln.on_hi[p] ? *reinterpret_cast<const R *>(x + ln.f_hi[p]) : zero;
         if (BWD) {
           const T *d = dp + (crow + hc) * D;
-          d_lo[p] = on_lo[p] && in ? *reinterpret_cast<const R *>(d + f_lo[p]) : zero;
-          d_hi[p] = on_hi[p] && in ? *reinterpret_cast<const R *>(d + f_hi[p]) : zero;
+          d_lo[p] = ln.on_lo[p] && in ? *reinterpret_cast<const R *>(d + ln.f_lo[p]) : zero;
+          d_hi[p] = ln.on_hi[p] && in ? *reinterpret_cast<const R *>(d + ln.f_hi[p]) : zero;
         }
       }
     };
@@ -191,124 +310,288 @@ __global__ void __launch_bounds__(kThreads) qk_norm_kernel(const __grid_constant
     for (int i = lane; i < tpw * half; i += 32) {
       const int ts = i / half, pr = i - ts * half;
       const long long tt = group * tpw + ts;
-      double turns = (double)position_of(a, tt < a.T ? tt : a.T - 1) * s_freq[pr];
-      turns -= rint(turns);
-      float sn, cs;
-      sincospif(2.f * (float)turns, &sn, &cs);
-      s_cos[warp][i] = cs;
-      s_sin[warp][i] = sn;
+      angle_of(position_of(a, tt < a.T ? tt : a.T - 1), s_freq[pr], s_cos[warp][i], s_sin[warp][i]);
     }
     __syncwarp();
     float cs[N], sn[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int p = i / VEC, j = i % VEC;
-      int pr = (p * LPR + gl) * VEC + j;   // the lane's i-th pair
-      if (INTER && VEC > 1)                // first half of the values: pairs of the low pack, then of the high pack
-        pr = ((j < VEC / 2 ? f_lo[p] : f_hi[p]) >> 1) + j % (VEC / 2 > 0 ? VEC / 2 : 1);
-      const bool rot = pr < half;
-      cs[i] = rot ? s_cos[warp][tsub * half + pr] : 1.f;
-      sn[i] = rot ? s_sin[warp][tsub * half + pr] : 0.f;
-    }
+    ln.angles(s_cos[warp] + tsub * half, s_sin[warp] + tsub * half, half, gl, BWD ? -1.f : 1.f, cs, sn);
     __syncwarp();  // the next item's angles overwrite these
 
     for (int hb = h0; hb < h1; hb += rpt) {
       const int h = hb + hsub;
       const bool live = t_on && h < h1;
-      float xl[N], xh[N], gl_[N], gh_[N];
+      float xl[N], xh[N], dl[N], dh[N];
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
         P::unpack(r_lo[p], xl + p * VEC);
         P::unpack(r_hi[p], xh + p * VEC);
         if (BWD) {
-          P::unpack(d_lo[p], gl_ + p * VEC);
-          P::unpack(d_hi[p], gh_ + p * VEC);
+          P::unpack(d_lo[p], dl + p * VEC);
+          P::unpack(d_hi[p], dh + p * VEC);
         }
       }
       if (hb + rpt < h1) fetch(h + rpt);
-      float s2 = 0.f;
-#pragma unroll
-      for (int i = 0; i < N; ++i) s2 += xl[i] * xl[i] + xh[i] * xh[i];
-      // (u, v) rotated by the i-th pair's angle (backward: by its negative)
-      auto rotate = [&](float *lo, float *hi) {
-        if (INTER && VEC > 1) {
-#pragma unroll
-          for (int p = 0; p < NP; ++p)
-#pragma unroll
-            for (int j = 0; j < VEC / 2; ++j) {
-              const int e = p * VEC + 2 * j, cl = p * VEC + j, ch = cl + VEC / 2;
-              const float s_l = BWD ? -sn[cl] : sn[cl], s_h = BWD ? -sn[ch] : sn[ch];
-              const float a0 = lo[e], a1 = lo[e + 1], b0 = hi[e], b1 = hi[e + 1];
-              lo[e] = a0 * cs[cl] - a1 * s_l;
-              lo[e + 1] = a1 * cs[cl] + a0 * s_l;
-              hi[e] = b0 * cs[ch] - b1 * s_h;
-              hi[e + 1] = b1 * cs[ch] + b0 * s_h;
-            }
-        } else {
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const float s = BWD ? -sn[i] : sn[i], u = lo[i], v = hi[i];
-            lo[i] = u * cs[i] - v * s;
-            hi[i] = v * cs[i] + u * s;
-          }
-        }
-      };
-      if (!BWD) {
-        const float rs = rsqrtf(lane_sum<LPR>(s2) + a.eps);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          xl[i] = xl[i] * rs * w_lo[i];
-          xh[i] = xh[i] * rs * w_hi[i];
-        }
-        rotate(xl, xh);
-      } else {
-        rotate(gl_, gh_);
-        float dot = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) dot += gl_[i] * w_lo[i] * xl[i] + gh_[i] * w_hi[i] * xh[i];
-        const float rs = rsqrtf(lane_sum<LPR>(s2) + a.eps);
-        dot = lane_sum<LPR>(dot) * rs;  // sum of g xh
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const float nl = xl[i] * rs, nh = xh[i] * rs;
-          dw_lo[i] += nl * gl_[i];
-          dw_hi[i] += nh * gh_[i];
-          xl[i] = (gl_[i] * w_lo[i] - nl * dot) * rs;
-          xh[i] = (gh_[i] * w_hi[i] - nh * dot) * rs;
-        }
-      }
+      if (BWD) ln.backward(xl, xh, dl, dh, cs, sn, a.eps, dw_lo, dw_hi);
+      else ln.forward(xl, xh, cs, sn, a.eps);
       if (live) {
         T *o = op + (crow + h) * D;
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
-          if (on_lo[p]) *reinterpret_cast<R *>(o + f_lo[p]) = P::pack(xl + p * VEC);
-          if (on_hi[p]) *reinterpret_cast<R *>(o + f_hi[p]) = P::pack(xh + p * VEC);
+          if (ln.on_lo[p]) *reinterpret_cast<R *>(o + ln.f_lo[p]) = P::pack(xl + p * VEC);
+          if (ln.on_hi[p]) *reinterpret_cast<R *>(o + ln.f_hi[p]) = P::pack(xh + p * VEC);
         }
       }
     }
   }
   if (BWD && a.partial[which] != nullptr) {  // uniform over the CTA
     __shared__ float part[kWarps][2 * LPR * N];
+    ln.leave(dw_lo, dw_hi, part, a.partial[which] + (long long)cta * D, a, warp, sub);
+  }
+}
+
+// ------------------------------------------------------------------------------ large calls
+constexpr int kDepth = 2;                                                      // slots of a warp's ring
+template <bool BWD> constexpr int slot_bytes() { return BWD ? 2048 : 4096; }  // of each tensor that is read
+template <bool BWD> constexpr int stream_smem() { return kWarps * kDepth * slot_bytes<BWD>() * (BWD ? 2 : 1); }
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// The rotation of a lane's N low and N high features as packed pairs of fp32, two neighbouring features each, out of the
+// token's cosines and sines in shared memory (16-byte pieces; pairs past the rotated ones are 1 and 0 there).
+//   lo' = lo a + {hi, or with INTER its own neighbour} b      hi' likewise with c and d
+// Forward with the weights multiplied in; back (BWD) without them, and a = c, b = -d where pairs are not neighbours.
+template <int N, bool INTER, bool BWD> struct Turn {
+  static constexpr int P = N / 2, Q = BWD && !INTER ? 0 : P;
+  float2 a[P], b[P], c[Q ? Q : 1], d[P];
+  __device__ __forceinline__ void set(const float *cs, const float *sn, int gl, int half_row, const float (&w_lo)[N],
+                                      const float (&w_hi)[N]) {
+    float co[N], si[N];
+    if (INTER) {  // N / 2 pairs of the low pack, N / 2 of the high one
+      read<P>(cs + gl * P, co);
+      read<P>(sn + gl * P, si);
+      read<P>(cs + half_row + gl * P, co + P);
+      read<P>(sn + half_row + gl * P, si + P);
+    } else {
+      read<N>(cs + gl * N, co);
+      read<N>(sn + gl * N, si);
+    }
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-#pragma unroll
-      for (int o = LPR; o < 32; o <<= 1) {
-        dw_lo[i] += __shfl_xor_sync(0xffffffffu, dw_lo[i], o);
-        dw_hi[i] += __shfl_xor_sync(0xffffffffu, dw_hi[i], o);
-      }
-      const int p = i / VEC, j = i % VEC;
-      if (sub == 0) {
-        if (on_lo[p]) part[warp][f_lo[p] + j] = dw_lo[i];
-        if (on_hi[p]) part[warp][f_hi[p] + j] = dw_hi[i];
+    for (int i = 0; i < P; ++i) {
+      const float l0 = BWD ? 1.f : w_lo[2 * i], l1 = BWD ? 1.f : w_lo[2 * i + 1];
+      const float h0 = BWD ? 1.f : w_hi[2 * i], h1 = BWD ? 1.f : w_hi[2 * i + 1];
+      if (INTER) {
+        const float cl = co[i], ch = co[i + P], sl = BWD ? -si[i] : si[i], sh = BWD ? -si[i + P] : si[i + P];
+        a[i] = make_float2(l0 * cl, l1 * cl);
+        b[i] = make_float2(-l1 * sl, l0 * sl);
+        c[Q ? i : 0] = make_float2(h0 * ch, h1 * ch);
+        d[i] = make_float2(-h1 * sh, h0 * sh);
+      } else {
+        const float s0 = BWD ? -si[2 * i] : si[2 * i], s1 = BWD ? -si[2 * i + 1] : si[2 * i + 1];
+        a[i] = make_float2(l0 * co[2 * i], l1 * co[2 * i + 1]);
+        b[i] = make_float2(-h0 * s0, -h1 * s1);
+        if (Q) c[Q ? i : 0] = make_float2(h0 * co[2 * i], h1 * co[2 * i + 1]);
+        d[i] = make_float2(l0 * s0, l1 * s1);
       }
     }
-    __syncthreads();
-    for (int f = threadIdx.x; f < D; f += kThreads) {
-      float s = 0.f;
+  }
+  __device__ __forceinline__ void apply(float2 (&lo)[P], float2 (&hi)[P]) const {
 #pragma unroll
-      for (int k = 0; k < kWarps; ++k) s += part[k][f];
-      a.partial[which][(long long)cta * D + f] = s * a.c;
+    for (int i = 0; i < P; ++i) {
+      const float2 u = lo[i], v = hi[i];
+      if (INTER) {
+        lo[i] = fma2(u, a[i], mul2(make_float2(u.y, u.x), b[i]));
+        hi[i] = fma2(v, c[Q ? i : 0], mul2(make_float2(v.y, v.x), d[i]));
+      } else {
+        lo[i] = fma2(u, a[i], mul2(v, b[i]));
+        hi[i] = fma2(v, Q ? c[Q ? i : 0] : a[i], mul2(u, d[i]));
+      }
     }
+  }
+  template <int W> static __device__ __forceinline__ void read(const float *p, float *v) {
+    if constexpr (W == 2) {
+      const float2 x = *reinterpret_cast<const float2 *>(p);
+      v[0] = x.x; v[1] = x.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; i += 4) {
+        const float4 x = *reinterpret_cast<const float4 *>(p + i);
+        v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w;
+      }
+    }
+  }
+};
+
+// A CTA owns a range of tokens, its warps take them in turn; a warp walks a token's heads in chunks of a.chunk rows = one
+// slot, one slot ahead.  Heads lie next to each other (D elements apart) and rows are a multiple of 16 bytes on
+// 16-byte boundaries.  The arithmetic is in packed pairs: with one fp32 operation an instruction the kernel issued 274 / 488
+// instructions for four rows of 128 features (forward / backward), 415 / 710 us for the call above; with 16 features a
+// lane it kept 16 warps an SM, which waited for shuffles and shared memory (376 / 691 us).
+template <typename T, bool BWD, bool INTER, int VEC, int LPR>
+__global__ void __launch_bounds__(kThreads, VEC == 8 ? 4 : (BWD ? 5 : 6)) qk_norm_stream_kernel(const __grid_constant__ QkArgs a, int *status) {
+  typedef Pack<T, VEC> P;
+  typedef typename P::R R;
+  constexpr int N = VEC, RPW = 32 / LPR, kSlot = slot_bytes<BWD>();
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ __align__(16) float s_cos[kWarps][LPR * N], s_sin[kWarps][LPR * N];
+  __shared__ double s_freq[kMaxD / 2];
+  __shared__ __align__(8) uint64_t bars[kWarps][kDepth];
+  __shared__ volatile int abort_flag;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int gl = lane % LPR, sub = lane / LPR;
+  const int which = blockIdx.x >= (unsigned)a.ctas[0];
+  const int cta = which ? blockIdx.x - a.ctas[0] : blockIdx.x;
+  const int H = a.heads[which], D = a.D, half = a.R >> 1;
+  for (int i = threadIdx.x; i < half; i += kThreads) s_freq[i] = a.freq[i];
+  for (int i = half + lane; i < LPR * N; i += 32) {  // pairs that pass
+    s_cos[warp][i] = 1.f;
+    s_sin[warp][i] = 0.f;
+  }
+  if (threadIdx.x == 0) abort_flag = 0;
+  if (lane < kDepth) ptx::mbar_init(ptx::smem_u32(&bars[warp][lane]), 1);
+  ptx::fence_barrier_init();
+  __syncthreads();
+  Lane<T, INTER, VEC, LPR, 1> ln;
+  ln.init(a, which, 0, gl);
+  float2 dw_lo[N / 2] = {}, dw_hi[N / 2] = {};
+  uint8_t *slots = ring + warp * kDepth * kSlot * (BWD ? 2 : 1);
+  const int chunk = a.chunk[which], chunks = a.chunks[which];
+  const int f_lo = ln.f_lo[0], f_hi = ln.f_hi[0];
+  const bool on = ln.on_lo[0];  // D is even: low and high features exist together
+  const long long t0 = a.T * cta / a.ctas[which] + warp, t1 = a.T * (cta + 1) / a.ctas[which];
+  const R zero = {};
+
+  // the next slot to fill: chunk fc of token ft = (fb, fn)
+  long long ft = t0, fb = t0 / a.N;
+  int fn = (int)(t0 - fb * a.N), fc = 0, fs = 0;
+  auto fill = [&]() {
+    if (ft >= t1) return;
+    if (lane == 0) {
+      const int h0 = fc * chunk;
+      const uint32_t bytes = (uint32_t)(min(chunk, H - h0) * D * (int)sizeof(T));
+      const uint32_t bar = ptx::smem_u32(&bars[warp][fs]), dst = ptx::smem_u32(slots + fs * kSlot * (BWD ? 2 : 1));
+      ptx::mbar_arrive_expect_tx(bar, BWD ? 2 * bytes : bytes);
+      bulk_load(dst, static_cast<const T *>(a.x[which]) + fb * a.sb[which] + fn * a.sn[which] + h0 * D, bytes, bar);
+      if (BWD) bulk_load(dst + kSlot, static_cast<const T *>(a.d_out[which]) + (ft * H + h0) * D, bytes, bar);
+    }
+    if (++fs == kDepth) fs = 0;
+    if (++fc == chunks) {
+      fc = 0;
+      ft += kWarps;
+      fn += kWarps;
+      while (fn >= a.N) {
+        fn -= a.N;
+        ++fb;
+      }
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kDepth - 1; ++i) fill();
+
+  int slot = 0, parity = 0;
+  bool ok = true;
+  long long b = t0 / a.N, doc0 = 0, doc1 = -1;  // sequence; the document a token was last found in
+  int n = (int)(t0 - b * a.N);
+  for (long long t = t0; t < t1 && ok; t += kWarps) {
+    long long position = n;
+    if (a.cu != nullptr) {
+      if (t >= doc1) {
+        int lo = 0, hi = a.M;  // largest i with cu[i] <= t
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (__ldg(a.cu + mid) <= t) lo = mid; else hi = mid - 1;
+        }
+        doc0 = __ldg(a.cu + lo);
+        doc1 = lo < a.M ? __ldg(a.cu + lo + 1) : a.T;
+      }
+      position = t - doc0;
+    } else if (a.pos != nullptr) {
+      position = __ldg(a.pos + b * a.pos_sb + n * a.pos_sn);
+    }
+    position += a.offset;
+    n += kWarps;
+    while (n >= a.N) {
+      n -= a.N;
+      ++b;
+    }
+    for (int i = lane; i < half; i += 32) angle_of(position, s_freq[i], s_cos[warp][i], s_sin[warp][i]);
+    __syncwarp();
+    Turn<N, INTER, BWD> turn;
+    turn.set(s_cos[warp], s_sin[warp], gl, D >> 2, ln.w_lo, ln.w_hi);
+    T *orow = static_cast<T *>(a.out[which]) + t * H * D;
+    for (int c = 0; c < chunks; ++c) {
+      fill();  // into the slot whose last reader has passed the barrier below
+      const int rows = min(chunk, H - c * chunk);
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bars[warp][slot]), parity, &abort_flag, status, 311));
+      if (!ok) break;
+      const T *xs = reinterpret_cast<const T *>(slots + slot * kSlot * (BWD ? 2 : 1));
+      const T *ds = reinterpret_cast<const T *>(slots + slot * kSlot * 2 + kSlot);
+      for (int r = sub; r - sub < rows; r += RPW) {
+        const bool live = r < rows;
+        const int at = (live ? r : rows - 1) * D;  // past the chunk: a row that exists, with a gradient of 0
+        float2 xl[N / 2], xh[N / 2];
+        P::unpack(on ? *reinterpret_cast<const R *>(xs + at + f_lo) : zero, reinterpret_cast<float *>(xl));
+        P::unpack(on ? *reinterpret_cast<const R *>(xs + at + f_hi) : zero, reinterpret_cast<float *>(xh));
+        float2 s2 = mul2(xl[0], xl[0]);
+        s2 = fma2(xh[0], xh[0], s2);
+#pragma unroll
+        for (int i = 1; i < N / 2; ++i) s2 = fma2(xh[i], xh[i], fma2(xl[i], xl[i], s2));
+        if (!BWD) {
+          const float2 rs = both(rsqrtf(lane_sum<LPR>(s2.x + s2.y) + a.eps));
+#pragma unroll
+          for (int i = 0; i < N / 2; ++i) {
+            xl[i] = mul2(xl[i], rs);
+            xh[i] = mul2(xh[i], rs);
+          }
+          turn.apply(xl, xh);
+        } else {
+          float2 dl[N / 2], dh[N / 2];
+          P::unpack(on && live ? *reinterpret_cast<const R *>(ds + at + f_lo) : zero, reinterpret_cast<float *>(dl));
+          P::unpack(on && live ? *reinterpret_cast<const R *>(ds + at + f_hi) : zero, reinterpret_cast<float *>(dh));
+          turn.apply(dl, dh);
+          const float2 *wl = reinterpret_cast<const float2 *>(ln.w_lo), *wh = reinterpret_cast<const float2 *>(ln.w_hi);
+          float2 dot = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int i = 0; i < N / 2; ++i) dot = fma2(mul2(dh[i], wh[i]), xh[i], fma2(mul2(dl[i], wl[i]), xl[i], dot));
+          const float rs1 = rsqrtf(lane_sum<LPR>(s2.x + s2.y) + a.eps);
+          const float2 rs = both(rs1), nd = both(-lane_sum<LPR>(dot.x + dot.y) * rs1);  // - sum of g xh
+#pragma unroll
+          for (int i = 0; i < N / 2; ++i) {
+            xl[i] = mul2(xl[i], rs);
+            xh[i] = mul2(xh[i], rs);
+            dw_lo[i] = fma2(xl[i], dl[i], dw_lo[i]);
+            dw_hi[i] = fma2(xh[i], dh[i], dw_hi[i]);
+            xl[i] = mul2(fma2(dl[i], wl[i], mul2(xl[i], nd)), rs);  // the product again: 16 registers less
+            xh[i] = mul2(fma2(dh[i], wh[i], mul2(xh[i], nd)), rs);
+          }
+        }
+        if (live && on) {
+          *reinterpret_cast<R *>(orow + at + f_lo) = P::pack(reinterpret_cast<const float *>(xl));
+          *reinterpret_cast<R *>(orow + at + f_hi) = P::pack(reinterpret_cast<const float *>(xh));
+        }
+      }
+      orow += chunk * D;
+      if (++slot == kDepth) {
+        slot = 0;
+        parity ^= 1;
+      }
+      __syncwarp();
+    }
+  }
+  if (!ok) {  // a wait gave up: let the copies in flight land
+    const uint64_t since = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - since < 1000000ull) __nanosleep(1000);
+  }
+  if (BWD && a.partial[which] != nullptr) {  // uniform over the CTA
+    __shared__ float part[kWarps][2 * LPR * N];
+    ln.leave(reinterpret_cast<float (&)[N]>(dw_lo), reinterpret_cast<float (&)[N]>(dw_hi), part,
+             a.partial[which] + (long long)cta * D, a, warp, sub);
   }
 }
 
@@ -345,8 +628,24 @@ int sm_count() {
   return sms[dev];
 }
 
+// CTAs in proportion to the rows of the tensors that have items, one at least, none without work
+void share_ctas(QkArgs &a, long long cap) {
+  const long long total = a.items[0] + a.items[1];
+  const long long rows = (a.items[0] ? a.heads[0] : 0) + (a.items[1] ? a.heads[1] : 0);
+  for (int k = 0; k < 2; ++k) {
+    const long long want = (a.items[k] + kWarps - 1) / kWarps;
+    long long n = want;
+    if (want > 0 && (total + kWarps - 1) / kWarps > cap) {
+      n = cap * a.heads[k] / rows;
+      if (n < 1) n = 1;
+      if (n > want) n = want;
+    }
+    a.ctas[k] = (int)(n < kMaxCtas / 2 ? n : kMaxCtas / 2);
+  }
+}
+
 template <typename T, bool BWD, bool INTER, int VEC, int LPR, int NP>
-int launch_cfg(QkArgs &a, int inter, cudaStream_t st) {
+int launch_cfg(QkArgs &a, int inter, const bool (&mine)[2], cudaStream_t st) {
   constexpr int RPW = 32 / LPR;
   const int sms = sm_count();
   if (sms <= 0) return LA_ERR_CUDA;
@@ -367,43 +666,103 @@ int launch_cfg(QkArgs &a, int inter, cudaStream_t st) {
     chunk = (chunk + rpt - 1) / rpt * rpt;
     a.chunk[k] = chunk;
     a.chunks[k] = (H + chunk - 1) / chunk;
-    a.items[k] = groups * a.chunks[k];
+    a.items[k] = mine[k] ? groups * a.chunks[k] : 0;
   }
-  // CTAs in proportion to the rows, one at least, none without work
-  const long long total = a.items[0] + a.items[1];
-  const long long cap = (long long)sms * resident;
-  for (int k = 0; k < 2; ++k) {
-    const long long want = (a.items[k] + kWarps - 1) / kWarps;
-    long long n = want;
-    if ((total + kWarps - 1) / kWarps > cap) {
-      n = cap * a.heads[k] / (a.heads[0] + a.heads[1]);
-      if (n < 1) n = 1;
-      if (n > want) n = want;
-    }
-    a.ctas[k] = (int)(n < kMaxCtas / 2 ? n : kMaxCtas / 2);
-  }
+  share_ctas(a, (long long)sms * resident);
   qk_norm_kernel<T, BWD, INTER, VEC, LPR, NP><<<a.ctas[0] + a.ctas[1], kThreads, 0, st>>>(a, inter);
   return launch_status();
 }
 
+template <typename T, bool BWD, bool INTER, int VEC, int LPR>
+int launch_stream(QkArgs &a, const bool (&mine)[2], cudaStream_t st) {
+  constexpr int RPW = 32 / LPR, kSmem = stream_smem<BWD>();
+  static bool set[64] = {false};
+  static int resident[64] = {0};
+  int dev = 0;
+  const int sms = sm_count();
+  if (sms <= 0 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return LA_ERR_CUDA;
+  if (!set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(qk_norm_stream_kernel<T, BWD, INTER, VEC, LPR>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e == cudaSuccess)
+      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident[dev], qk_norm_stream_kernel<T, BWD, INTER, VEC, LPR>,
+                                                        kThreads, kSmem);
+    if (e != cudaSuccess || resident[dev] < 1) {
+      note_cuda_error(e, "qk_norm shared memory");
+      return LA_ERR_CUDA;
+    }
+    set[dev] = true;
+  }
+  for (int k = 0; k < 2; ++k) {
+    int chunk = slot_bytes<BWD>() / (a.D * (int)sizeof(T)) / RPW * RPW;
+    if (chunk > a.heads[k]) chunk = a.heads[k];
+    a.chunk[k] = chunk;
+    a.chunks[k] = (a.heads[k] + chunk - 1) / chunk;
+    a.items[k] = mine[k] ? a.T : 0;
+  }
+  share_ctas(a, (long long)sms * resident[dev]);
+  qk_norm_stream_kernel<T, BWD, INTER, VEC, LPR><<<a.ctas[0] + a.ctas[1], kThreads, kSmem, st>>>(a, status_word_ptr());
+  return launch_status();
+}
+
+// Streamed: tensors whose heads lie next to each other and fill a warp's rows, from 2^20 elements on.  Measured, forward /
+// backward in us, streamed against direct: 16 heads of 128 (bf16), 2^18 elements 5.0 / 9.1 against 4.8 / 8.8, 2^20
+// 5.6 / 10.7 against 8.8 / 16.5, 2^24 28 / 44 against 40 / 75; 32 heads of 128 (fp32), 2^18 8.3 / 14.4 against 4.3 / 8.2,
+// 2^20 8.5 / 15.3 against 9.1 / 14.3, 2^23 27 / 44 against 29 / 46.
+template <typename T, bool BWD, bool INTER, int VEC, int LPR>
+int launch_both(QkArgs &a, cudaStream_t st) {
+  // streamed 16-bit rows are taken in 8-byte pieces: half the features, and so half the registers, a lane
+  constexpr bool kHalf = VEC == 8 && LPR <= 16;
+  constexpr int SVEC = kHalf ? 4 : VEC, SLPR = kHalf ? 2 * LPR : LPR, RPW = 32 / SLPR;
+  constexpr int kPer = 16 / (int)sizeof(T);
+  bool stream[2], direct[2];
+  for (int k = 0; k < 2; ++k) {
+    const bool on16 = (reinterpret_cast<uintptr_t>(a.x[k]) | reinterpret_cast<uintptr_t>(a.d_out[k])) % 16 == 0 &&
+                      a.D % kPer == 0 && a.sb[k] % kPer == 0 && a.sn[k] % kPer == 0;
+    stream[k] = on16 && a.heads[k] >= RPW && (a.heads[k] == 1 || a.sh[k] == a.D) &&
+                RPW * a.D * (int)sizeof(T) <= slot_bytes<BWD>() && a.T * a.heads[k] * a.D >= kStreamFrom;
+    direct[k] = !stream[k];
+  }
+  int ctas[2] = {0, 0}, rc = LA_OK;
+  if (stream[0] || stream[1]) {
+    rc = launch_stream<T, BWD, INTER, SVEC, SLPR>(a, stream, st);
+    ctas[0] = a.ctas[0];
+    ctas[1] = a.ctas[1];
+  }
+  if (rc == LA_OK && (direct[0] || direct[1])) {
+    rc = launch_cfg<T, BWD, INTER, VEC, LPR, 1>(a, INTER, direct, st);
+    ctas[0] += a.ctas[0];
+    ctas[1] += a.ctas[1];
+  }
+  a.ctas[0] = ctas[0];  // partial rows of each tensor
+  a.ctas[1] = ctas[1];
+  return rc;
+}
+
 template <typename T, bool BWD, bool INTER, int VEC>
 int launch_vec(QkArgs &a, int inter, cudaStream_t st) {
+  const bool both[2] = {true, true};
   const int lanes = ((a.D + 1) / 2 + VEC - 1) / VEC;
   if constexpr (VEC == 1) {
-    if (lanes <= 32) return launch_cfg<T, BWD, false, 1, 32, 1>(a, inter, st);
-    if (lanes <= 64) return launch_cfg<T, BWD, false, 1, 32, 2>(a, inter, st);
-    if (lanes <= 128) return launch_cfg<T, BWD, false, 1, 32, 4>(a, inter, st);
-    return launch_cfg<T, BWD, false, 1, 32, 8>(a, inter, st);
-  } else {
+    if (lanes <= 32) return launch_cfg<T, BWD, false, 1, 32, 1>(a, inter, both, st);
+    if (lanes <= 64) return launch_cfg<T, BWD, false, 1, 32, 2>(a, inter, both, st);
+    if (lanes <= 128) return launch_cfg<T, BWD, false, 1, 32, 4>(a, inter, both, st);
+    return launch_cfg<T, BWD, false, 1, 32, 8>(a, inter, both, st);
+  } else if constexpr (VEC * sizeof(T) == 16) {
     if constexpr (VEC == 8) {
-      if (lanes <= 2) return launch_cfg<T, BWD, INTER, VEC, 2, 1>(a, inter, st);
+      if (lanes <= 2) return launch_both<T, BWD, INTER, VEC, 2>(a, st);
     }
-    if (lanes <= 4) return launch_cfg<T, BWD, INTER, VEC, 4, 1>(a, inter, st);
-    if (lanes <= 8) return launch_cfg<T, BWD, INTER, VEC, 8, 1>(a, inter, st);
-    if (lanes <= 16) return launch_cfg<T, BWD, INTER, VEC, 16, 1>(a, inter, st);
-    if (lanes <= 32) return launch_cfg<T, BWD, INTER, VEC, 32, 1>(a, inter, st);
-    if constexpr (VEC == 4) return launch_cfg<T, BWD, INTER, VEC, 32, 2>(a, inter, st);
+    if (lanes <= 4) return launch_both<T, BWD, INTER, VEC, 4>(a, st);
+    if (lanes <= 8) return launch_both<T, BWD, INTER, VEC, 8>(a, st);
+    if (lanes <= 16) return launch_both<T, BWD, INTER, VEC, 16>(a, st);
+    if (lanes <= 32) return launch_both<T, BWD, INTER, VEC, 32>(a, st);
+    if constexpr (VEC == 4) return launch_cfg<T, BWD, INTER, VEC, 32, 2>(a, inter, both, st);
     return LA_ERR_UNSUPPORTED;
+  } else {  // 8-byte accesses of 16-bit types
+    if (lanes <= 8) return launch_cfg<T, BWD, INTER, VEC, 8, 1>(a, inter, both, st);
+    if (lanes <= 16) return launch_cfg<T, BWD, INTER, VEC, 16, 1>(a, inter, both, st);
+    if (lanes <= 32) return launch_cfg<T, BWD, INTER, VEC, 32, 1>(a, inter, both, st);
+    return launch_cfg<T, BWD, INTER, VEC, 32, 2>(a, inter, both, st);
   }
 }
 
