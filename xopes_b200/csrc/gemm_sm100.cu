@@ -430,8 +430,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kCols) : "memory");
 }
 
-// (outer, inner) matrix of 16-bit elements, inner next to each other, rows `ld` elements apart; boxes of 64 inner
-// elements (128 bytes, swizzled) by `rows` outer ones, zeros outside.
+}  // namespace
+
 int make_map_2d(CUtensorMap *m, const void *p, int dtype, int64_t inner, int64_t outer, int64_t ld, int rows) {
   tile::EncodeTiledFn enc = tile::encode_fn();
   if (enc == nullptr) return LA_ERR_CUDA;
@@ -453,6 +453,9 @@ int make_map_2d(CUtensorMap *m, const void *p, int dtype, int64_t inner, int64_t
              (long long)outer, (long long)inner, (long long)ld);
   return r == CUDA_SUCCESS ? LA_OK : LA_ERR_CUDA;
 }
+
+namespace {
+
 int operand_map(CUtensorMap *m, const Operand &o, int dtype, int64_t R, int64_t K, int rows) {
   return o.mn_major ? make_map_2d(m, o.p, dtype, R, K, o.ld, kStepK) : make_map_2d(m, o.p, dtype, K, R, o.ld, rows);
 }

@@ -425,6 +425,10 @@ int readable(Operand &o, int64_t rows, int64_t cols, int dtype, Scratch &s, cuda
 
 // One product with its epilogue.  With s.base null only the scratch is counted.
 int product(Product p, int dtype, Scratch s, int64_t &need, cudaStream_t st) {
+  if (few_tokens_fit(p, dtype)) {
+    if (s.used > need) need = s.used;
+    return s.base == nullptr ? LA_OK : few_tokens_launch(p, dtype, st);
+  }
   GemmPlan plan = {0, 1};
   if (dtype == LA_F32) {
     const int64_t k = p.K[0] + (p.segments > 1 ? p.K[1] : 0);

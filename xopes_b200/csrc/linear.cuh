@@ -2,6 +2,8 @@
 // (bias, activation, product of the pair, residual), and the interface between the host plan (linear.cu) and the
 // matrix kernels (gemm_sm100.cu).
 #pragma once
+#include <cuda.h>
+
 #include "common.cuh"
 
 namespace la {
@@ -302,6 +304,14 @@ struct GemmPlan {
 };
 GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K0, int64_t K1, bool pair);
 int gemm_launch(const Product &p, const GemmPlan &plan, float *partial, int dtype, cudaStream_t st);
+
+// Tensor map of an (outer, inner) matrix of 16-bit elements, inner next to each other, rows `ld` elements apart; boxes of 64
+// inner elements (128 bytes, swizzled) by `rows` outer ones, zeros outside.
+int make_map_2d(CUtensorMap *m, const void *p, int dtype, int64_t inner, int64_t outer, int64_t ld, int rows);
+
+// few_tokens.cu: whether a product is its kind, and the launch (same alignment).
+bool few_tokens_fit(const Product &p, int dtype);
+int few_tokens_launch(const Product &p, int dtype, cudaStream_t st);
 
 }  // namespace lin
 }  // namespace la
