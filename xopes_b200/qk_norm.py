@@ -23,27 +23,55 @@ def _frequencies(base: float, rotary_dim: int):
     return (ctypes.c_double * max(n, 1))(*[base ** (-2.0 * i / rotary_dim) for i in range(n)])
 
 
+def _forward(q, k, q_weight, k_weight, positions, offset, cu, freq, rotary_dim, interleaved, c, eps):
+    """The outputs, and q and k as the kernel read them (features next to each other)."""
+    lib = _lib.load()
+    b, n, h, d = q.shape
+    hk = k.shape[2]
+    q_sb, q_sn, q_sh, one = q.stride()
+    if one != 1 and d > 1:
+        q = q.contiguous()
+        q_sb, q_sn, q_sh, _ = q.stride()
+    k_sb, k_sn, k_sh, one = k.stride()
+    if one != 1 and d > 1:
+        k = k.contiguous()
+        k_sb, k_sn, k_sh, _ = k.stride()
+    wq, wk, wcode = _weights(q, q_weight, k_weight)
+    qo = torch.empty((b, n, h, d), dtype=q.dtype, device=q.device)
+    ko = torch.empty((b, n, hk, d), dtype=q.dtype, device=q.device)
+    pos, pos_sb, pos_sn = _positions(positions)
+    with _lib.device_of(q):
+        rc = lib.la_qk_norm_rope_fwd(
+            q.data_ptr(), q_sb, q_sn, q_sh, k.data_ptr(), k_sb, k_sn, k_sh, _lib.ptr(wq), _lib.ptr(wk), wcode, pos, pos_sb,
+            pos_sn, offset, _lib.ptr(cu), 0 if cu is None else cu.numel() - 1, freq, qo.data_ptr(), ko.data_ptr(), b, n, h, hk,
+            d, rotary_dim, _lib.dtype_code(q), interleaved, c, eps, _lib.stream_of(q))
+    if rc:
+        _lib.check(rc, "la_qk_norm_rope_fwd")
+    return qo, ko, q, k
+
+
+def _positions(positions):
+    if positions is None:
+        return None, 0, 0
+    return positions.data_ptr(), positions.stride(0) if positions.shape[0] > 1 else 0, positions.stride(1)
+
+
+def _weights(q, q_weight, k_weight):
+    """The weights in one type the kernel reads: both of q's type, or fp32."""
+    dt = q.dtype
+    if (q_weight is not None and q_weight.dtype != dt) or (k_weight is not None and k_weight.dtype != dt):
+        dt = torch.float32
+    wq = None if q_weight is None else q_weight.to(dt).contiguous()
+    wk = None if k_weight is None else k_weight.to(dt).contiguous()
+    return wq, wk, _lib.LA_F32 if dt == torch.float32 else _lib.dtype_code(q)
+
+
 class QkNormRopeFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, offset, cu, freq, rotary_dim, interleaved, c, eps):
-        lib = _lib.load()
-        q, k = (t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous() for t in (q, k))
-        b, n, h, d = q.shape
-        hk = k.shape[2]
-        wq, wk, wcode = _weights(q, q_weight, k_weight)
-        qo = torch.empty(b, n, h, d, dtype=q.dtype, device=q.device)
-        ko = torch.empty(b, n, hk, d, dtype=q.dtype, device=q.device)
-        pos_sb, pos_sn = (0, 0) if positions is None else (positions.stride(0) if positions.shape[0] > 1 else 0,
-                                                           positions.stride(1))
-        m = 0 if cu is None else cu.numel() - 1
-        with _lib.device_of(q):
-            rc = lib.la_qk_norm_rope_fwd(
-                _lib.ptr(q), *q.stride()[:3], _lib.ptr(k), *k.stride()[:3], _lib.ptr(wq), _lib.ptr(wk), wcode,
-                _lib.ptr(positions), pos_sb, pos_sn, offset, _lib.ptr(cu), m, freq, _lib.ptr(qo), _lib.ptr(ko),
-                b, n, h, hk, d, rotary_dim, _lib.dtype_code(q), interleaved, c, eps, _lib.stream_of(q))
-        _lib.check(rc, "la_qk_norm_rope_fwd")
+        qo, ko, q, k = _forward(q, k, q_weight, k_weight, positions, offset, cu, freq, rotary_dim, interleaved, c, eps)
         ctx.save_for_backward(q, k, q_weight, k_weight, positions, cu)
-        ctx.cfg = (offset, freq, rotary_dim, interleaved, c, eps, pos_sb, pos_sn)
+        ctx.cfg = (offset, freq, rotary_dim, interleaved, c, eps)
         ctx.set_materialize_grads(False)
         return qo, ko
 
@@ -51,7 +79,8 @@ class QkNormRopeFunction(torch.autograd.Function):
     def backward(ctx, dqo, dko):
         lib = _lib.load()
         q, k, q_weight, k_weight, positions, cu = ctx.saved_tensors
-        offset, freq, rotary_dim, interleaved, c, eps, pos_sb, pos_sn = ctx.cfg
+        offset, freq, rotary_dim, interleaved, c, eps = ctx.cfg
+        pos, pos_sb, pos_sn = _positions(positions)
         b, n, h, d = q.shape
         hk = k.shape[2]
         dqo = torch.zeros(b, n, h, d, dtype=q.dtype, device=q.device) if dqo is None else dqo.to(q.dtype).contiguous()
@@ -69,20 +98,12 @@ class QkNormRopeFunction(torch.autograd.Function):
         with _lib.device_of(q):
             rc = lib.la_qk_norm_rope_bwd(
                 _lib.ptr(q), *q.stride()[:3], _lib.ptr(k), *k.stride()[:3], _lib.ptr(wq), _lib.ptr(wk), wcode,
-                _lib.ptr(positions), pos_sb, pos_sn, offset, _lib.ptr(cu), m, freq, _lib.ptr(dqo), _lib.ptr(dko),
+                pos, pos_sb, pos_sn, offset, _lib.ptr(cu), m, freq, _lib.ptr(dqo), _lib.ptr(dko),
                 _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dwq), _lib.ptr(dwk), _lib.ptr(ws), ws_bytes,
                 b, n, h, hk, d, rotary_dim, _lib.dtype_code(q), interleaved, c, eps, _lib.stream_of(q))
         _lib.check(rc, "la_qk_norm_rope_bwd")
         return (dq, dk, None if dwq is None else dwq.to(q_weight.dtype), None if dwk is None else dwk.to(k_weight.dtype),
                 None, None, None, None, None, None, None, None)
-
-
-def _weights(q, q_weight, k_weight):
-    """The weights in one type the kernel reads: both of q's type, or fp32."""
-    given = [w.dtype for w in (q_weight, k_weight) if w is not None]
-    dt = q.dtype if given and all(t == q.dtype for t in given) else torch.float32
-    wq, wk = (None if w is None else w.detach().to(dt).contiguous() for w in (q_weight, k_weight))
-    return wq, wk, _lib.dtype_code(q) if dt == q.dtype else _lib.LA_F32
 
 
 def qk_norm_rope_fn(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
@@ -107,9 +128,9 @@ def qk_norm_rope_fn(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.T
     if q.dtype != k.dtype:
         raise TypeError(f"q and k must have one dtype, got {q.dtype} and {k.dtype}")
     b, n, _, d = q.shape
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and tuple(w.shape) != (d,):
-            raise ValueError(f"{name} must have shape ({d},), got {tuple(w.shape)}")
+    for w in (q_weight, k_weight):
+        if w is not None and w.shape != (d,):
+            raise ValueError(f"q_weight and k_weight must have shape ({d},), got {tuple(w.shape)}")
     r = d - d % 2 if rotary_dim is None else int(rotary_dim)
     if r < 0 or r > d or r % 2:
         raise ValueError(f"rotary_dim must be even and between 0 and {d}, got {rotary_dim}")
@@ -132,10 +153,13 @@ def qk_norm_rope_fn(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.T
             positions = positions[None]
         if positions.dim() != 2 or positions.shape[0] not in (1, b) or positions.shape[1] != n:
             raise ValueError(f"positions must have shape ({b},{n}), (1,{n}) or ({n},), got {tuple(positions.shape)}")
-    _lib.require_cuda(q, k, q_weight, k_weight, positions, cu_seqlens)
+    device, grad = q.device, q.requires_grad
     for t in (k, q_weight, k_weight, positions, cu_seqlens):
-        if t is not None and t.device != q.device:
-            raise ValueError(f"all tensors must be on {q.device}, got one on {t.device}")
+        if t is not None:
+            if t.device != device:
+                raise ValueError(f"all tensors must be on {device}, got one on {t.device}")
+            grad = grad or t.requires_grad
+    _lib.require_cuda(q)
     cu = None
     if cu_seqlens is not None:
         if b != 1:
@@ -144,5 +168,7 @@ def qk_norm_rope_fn(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.T
     _lib.dtype_code(q)
     if q.numel() == 0 or k.numel() == 0:
         raise ValueError("q and k must have at least one element")
-    return QkNormRopeFunction.apply(q, k, q_weight, k_weight, positions, int(offset), cu, freq, r, int(bool(interleaved)),
-                                    float(c), float(eps))
+    args = (q, k, q_weight, k_weight, positions, int(offset), cu, freq, r, 1 if interleaved else 0, float(c), float(eps))
+    if grad and torch.is_grad_enabled():
+        return QkNormRopeFunction.apply(*args)
+    return _forward(*args)[:2]
