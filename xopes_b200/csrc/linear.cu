@@ -42,7 +42,6 @@ struct SimtArgs {
   Operand a[2], b[2];
   long long K[2];
   int vec_a[2], vec_b[2];
-  int segments;
   long long M, N;
   int n_tiles, splits;
   long long steps[2];  // 16-wide steps of each segment
@@ -50,47 +49,56 @@ struct SimtArgs {
   Epilogue e;
 };
 
-constexpr int kTile = 64, kStep = 16, kPitch = kTile + 4;
+constexpr int kTile = 64, kStep = 16, kPitch = kTile + 4, kSimtThreads = 128;
 
-// four elements of a 64 x 16 operand tile for this thread: along the contraction, or along the rows (mn_major)
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+
+// eight elements of a 64 x 16 operand tile for this thread, two quads: along the contraction, or along the rows (mn_major)
 __device__ __forceinline__ void simt_fetch(const Operand &o, int vec, long long r0, long long R, long long k0, long long K,
-                                           float (&v)[4]) {
+                                           float (&v)[8]) {
   const int t = threadIdx.x;
   const float *p = static_cast<const float *>(o.p);
-  if (!o.mn_major) {
-    const long long r = r0 + (t >> 2), k = k0 + (t & 3) * 4;
-    if (r < R) load_row<float, 4>(p + r * o.ld + k, vec, (int)(K - k < 4 ? K - k : 4), v);
-    else v[0] = v[1] = v[2] = v[3] = 0.f;
-  } else {
-    const long long k = k0 + (t >> 4), r = r0 + (t & 15) * 4;
-    if (k < K) load_row<float, 4>(p + k * o.ld + r, vec, (int)(R - r < 4 ? R - r : 4), v);
-    else v[0] = v[1] = v[2] = v[3] = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float (&q)[4] = reinterpret_cast<float (&)[4]>(v[4 * i]);
+    q[0] = q[1] = q[2] = q[3] = 0.f;
+    if (!o.mn_major) {
+      const long long r = r0 + (t >> 2) + 32 * i, k = k0 + (t & 3) * 4;
+      if (r < R) load_row<float, 4>(p + r * o.ld + k, vec, (int)(K - k < 4 ? K - k : 4), q);
+    } else {
+      const long long k = k0 + (t >> 4) + 8 * i, r = r0 + (t & 15) * 4;
+      if (k < K) load_row<float, 4>(p + k * o.ld + r, vec, (int)(R - r < 4 ? R - r : 4), q);
+    }
   }
 }
-__device__ __forceinline__ void simt_put(const Operand &o, float (*s)[kPitch], const float (&v)[4]) {
+__device__ __forceinline__ void simt_put(const Operand &o, float (*s)[kPitch], const float (&v)[8]) {
   const int t = threadIdx.x;
-  if (!o.mn_major) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[(t & 3) * 4 + j][t >> 2] = v[j];
-  } else {
+  for (int i = 0; i < 2; ++i) {
+    if (!o.mn_major) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[t >> 4][(t & 15) * 4 + j] = v[j];
+      for (int j = 0; j < 4; ++j) s[(t & 3) * 4 + j][(t >> 2) + 32 * i] = v[4 * i + j];
+    } else {
+      *reinterpret_cast<float4 *>(&s[(t >> 4) + 8 * i][(t & 15) * 4]) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    }
   }
 }
 
-// One 64 x 64 tile (of one split) per CTA of 256 threads, 4 x 4 results a thread; the next step's operands are in
-// registers while the current step's are multiplied.
+// One 64 x 64 tile (of one split) per CTA of 128 threads, 8 x 4 results a thread, packed over pairs of rows; the next step's
+// operands are in registers while the current step's are multiplied.  514 x 512 x 512 17 us with the sum of the splits,
+// 2048 x 2048 x 2048 436 us (39 TFLOP/s; fp32 units and the instructions beside the products bound it; elements of B kept twice
+// in shared memory, to save the doubling, made shared memory the bound: 860 us).
 template <bool PAIR>
-__global__ void __launch_bounds__(256) simt_product_kernel(const SimtArgs a) {
-  __shared__ __align__(16) float sa[kStep][kPitch], sb[PAIR ? 2 : 1][kStep][kPitch];
+__global__ void __launch_bounds__(kSimtThreads) simt_product_kernel(const SimtArgs a) {
+  __shared__ __align__(16) float sa[2][kStep][kPitch], sb[2][PAIR ? 2 : 1][kStep][kPitch];
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const long long tile = blockIdx.x / a.splits;
   const int split = (int)(blockIdx.x - tile * a.splits);
   const long long m0 = tile / a.n_tiles * kTile, n0 = tile % a.n_tiles * kTile;
   const long long all = a.steps[0] + a.steps[1];
   const long long s0 = all * split / a.splits, s1 = all * (split + 1) / a.splits;
-  float acc[4][4] = {}, acc2[PAIR ? 4 : 1][4] = {};
-  float va[4], vb[4], vb2[4];
+  float2 acc[4][4] = {}, acc2[PAIR ? 4 : 1][4] = {};  // rows 2 i and 2 i + 1, column j
+  float va[8], vb[8], vb2[8];
   auto fetch = [&](long long s) {
     const int g = s >= a.steps[0];
     const long long k0 = (g ? s - a.steps[0] : s) * kStep;
@@ -98,50 +106,133 @@ __global__ void __launch_bounds__(256) simt_product_kernel(const SimtArgs a) {
     simt_fetch(a.b[g], a.vec_b[g], n0, a.N, k0, a.K[g], vb);
     if (PAIR) simt_fetch(a.b[1], a.vec_b[1], n0, a.N, k0, a.K[0], vb2);
   };
-  if (s0 < s1) fetch(s0);
-  for (long long s = s0; s < s1; ++s) {
+  auto put = [&](long long s, int at) {
     const int g = s >= a.steps[0];
-    __syncthreads();
-    simt_put(a.a[g], sa, va);
-    simt_put(a.b[g], sb[0], vb);
-    if (PAIR) simt_put(a.b[1], sb[PAIR ? 1 : 0], vb2);
-    __syncthreads();
+    simt_put(a.a[g], sa[at], va);
+    simt_put(a.b[g], sb[at][0], vb);
+    if (PAIR) simt_put(a.b[1], sb[at][PAIR ? 1 : 0], vb2);
+  };
+  if (s0 < s1) {
+    fetch(s0);
+    put(s0, 0);
+  }
+  __syncthreads();
+  for (long long s = s0; s < s1; ++s) {
+    const int at = (int)(s - s0) & 1;
     if (s + 1 < s1) fetch(s + 1);
 #pragma unroll
     for (int k = 0; k < kStep; ++k) {
-      const float4 x = *reinterpret_cast<const float4 *>(&sa[k][ty * 4]);
-      const float4 y = *reinterpret_cast<const float4 *>(&sb[0][k][tx * 4]);
-      const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+      float2 x[4];
+      float y[4];
+      *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(&sa[at][k][ty * 8]);
+      *reinterpret_cast<float4 *>(x + 2) = *reinterpret_cast<const float4 *>(&sa[at][k][ty * 8 + 4]);
+      *reinterpret_cast<float4 *>(y) = *reinterpret_cast<const float4 *>(&sb[at][0][k][tx * 4]);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += xs[i] * ys[j];
+        for (int j = 0; j < 4; ++j) acc[i][j] = fma2(x[i], make_float2(y[j], y[j]), acc[i][j]);
       if (PAIR) {
-        const float4 z = *reinterpret_cast<const float4 *>(&sb[PAIR ? 1 : 0][k][tx * 4]);
-        const float zs[4] = {z.x, z.y, z.z, z.w};
+        *reinterpret_cast<float4 *>(y) = *reinterpret_cast<const float4 *>(&sb[at][PAIR ? 1 : 0][k][tx * 4]);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc2[PAIR ? i : 0][j] += xs[i] * zs[j];
+          for (int j = 0; j < 4; ++j) acc2[PAIR ? i : 0][j] = fma2(x[i], make_float2(y[j], y[j]), acc2[PAIR ? i : 0][j]);
       }
     }
+    if (s + 1 < s1) put(s + 1, at ^ 1);
+    __syncthreads();
   }
   const long long n = n0 + tx * 4;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long m = m0 + ty * 4 + i;
+  for (int i = 0; i < 8; ++i) {
+    const long long m = m0 + ty * 8 + i;
     if (m >= a.M || n >= a.N) continue;
+    float p[4], q[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      p[j] = i % 2 ? acc[i / 2][j].y : acc[i / 2][j].x;
+      q[j] = i % 2 ? acc2[PAIR ? i / 2 : 0][j].y : acc2[PAIR ? i / 2 : 0][j].x;
+    }
     if (a.partial != nullptr) {
-      float *p = a.partial + ((long long)split * (PAIR ? 2 : 1) * a.M + m) * a.N + n;
+      float *o = a.partial + ((long long)split * (PAIR ? 2 : 1) * a.M + m) * a.N + n;
       const int left = (int)(a.N - n < 4 ? a.N - n : 4);
-      store_row<float, 4>(p, a.N % 4 == 0, left, acc[i]);
-      if (PAIR) store_row<float, 4>(p + a.M * a.N, a.N % 4 == 0, left, acc2[PAIR ? i : 0]);
+      store_row<float, 4>(o, a.N % 4 == 0, left, p);
+      if (PAIR) store_row<float, 4>(o + a.M * a.N, a.N % 4 == 0, left, q);
     } else if (PAIR) {
-      finish_pair<float, 4>(a.e, m, (int)n, (int)a.N, acc[i], acc2[PAIR ? i : 0]);
+      finish_pair<float, 4>(a.e, m, (int)n, (int)a.N, p, q);
     } else {
-      finish_one<float, 4>(a.e, m, (int)n, (int)a.N, acc[i]);
+      finish_one<float, 4>(a.e, m, (int)n, (int)a.N, p);
     }
   }
+}
+
+// Up to 8 tokens in fp32: the weights' bytes are the work.  A warp streams four weight rows (two of each of a pair) and keeps
+// their products with MT tokens; `share` warps of the CTA split the contraction.  At the end a butterfly that halves the
+// values at every step leaves lane i with value i.  1 / 8 tokens, 4096 x 4096: 14.3 / 31 us; 10.3 of weights at
+// the measured copy bandwidth.
+template <int MT, bool PAIR>
+__global__ void __launch_bounds__(256) few_tokens_fp32_kernel(const float *x, long long ldx, const float *w0, long long ldw0,
+                                                              const float *w1, long long ldw1, int M, int N, int K,
+                                                              int share, Epilogue e) {
+  constexpr int kRows = PAIR ? 2 : 4, V = 4 * MT;
+  __shared__ float part[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int at = warp % share;
+  const long long n0 = ((long long)blockIdx.x * 8 + warp) / share * kRows;
+  const float *w[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const long long n = n0 + r % kRows < N ? n0 + r % kRows : N - 1;
+    w[r] = PAIR && r >= 2 ? w1 + n * ldw1 : w0 + n * ldw0;
+  }
+  float2 acc[4][MT] = {};
+#pragma unroll 2
+  for (int k = (at * 32 + lane) * 4; k < K; k += share * 128) {
+    float4 v[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = *reinterpret_cast<const float4 *>(w[r] + k);
+    float4 t[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) t[m] = *reinterpret_cast<const float4 *>(x + (m < M ? m : M - 1) * ldx + k);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        acc[r][m] = fma2(make_float2(v[r].z, v[r].w), make_float2(t[m].z, t[m].w),
+                         fma2(make_float2(v[r].x, v[r].y), make_float2(t[m].x, t[m].y), acc[r][m]));
+  }
+  float s[V];
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) s[r * MT + m] = acc[r][m].x + acc[r][m].y;
+  int off = 16;
+#pragma unroll
+  for (int n = V; n > 1; n /= 2, off /= 2) {
+    const bool up = lane & off;
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j)
+      if (j < n / 2) {
+        const float give = up ? s[j] : s[j + n / 2], keep = up ? s[j + n / 2] : s[j];
+        s[j] = keep + __shfl_xor_sync(0xffffffffu, give, off);
+      }
+  }
+#pragma unroll
+  for (; off > 0; off /= 2) s[0] += __shfl_xor_sync(0xffffffffu, s[0], off);
+  constexpr int kStride = 32 / V;  // lanes that hold one value
+  if (lane % kStride == 0) part[warp][lane / kStride] = s[0];
+  __syncthreads();
+  if (at != 0 || lane >= (PAIR ? V / 2 : V)) return;
+  float p[1] = {0.f}, q[1] = {0.f};
+  for (int i = 0; i < share; ++i) {
+    p[0] += part[warp + i][lane];
+    if (PAIR) q[0] += part[warp + i][lane + V / 2];
+  }
+  const int m = lane % MT;
+  const long long n = n0 + lane / MT;
+  if (m >= M || n >= N) return;
+  if (PAIR) finish_pair<float, 1>(e, m, (int)n, N, p, q);
+  else finish_one<float, 1>(e, m, (int)n, N, p);
 }
 
 // ------------------------------------------------------------------------------ sums over the splits
@@ -377,7 +468,6 @@ int epilogue_vec(const Epilogue &e, int dtype) {
 
 int simt_launch(const Product &p, int splits, float *partial, cudaStream_t st) {
   SimtArgs a = {};
-  a.segments = p.segments;
   a.M = p.M; a.N = p.N; a.e = p.e;
   for (int s = 0; s < 2; ++s) {
     a.a[s] = p.a[s]; a.b[s] = p.b[s];
@@ -392,8 +482,32 @@ int simt_launch(const Product &p, int splits, float *partial, cudaStream_t st) {
   a.partial = partial;
   const int64_t grid = mt * a.n_tiles * splits;
   if (grid > INT32_MAX) return LA_ERR_TOO_LARGE;
-  if (p.pair) simt_product_kernel<true><<<(unsigned)grid, 256, 0, st>>>(a);
-  else simt_product_kernel<false><<<(unsigned)grid, 256, 0, st>>>(a);
+  if (p.pair) simt_product_kernel<true><<<(unsigned)grid, kSimtThreads, 0, st>>>(a);
+  else simt_product_kernel<false><<<(unsigned)grid, kSimtThreads, 0, st>>>(a);
+  return launch_status();
+}
+
+// Whether a product is few_tokens_fp32_kernel's kind, and the launch: enough warps to fill the GPU, each with 256 terms.
+bool few_fp32_fit(const Product &p) {
+  auto on16 = [](const Operand &o) { return !o.mn_major && aligned16(o.p) && o.ld % 4 == 0; };
+  return p.M <= 8 && p.segments == 1 && p.K[0] % 4 == 0 && on16(p.a[0]) && on16(p.b[0]) && (!p.pair || on16(p.b[1]));
+}
+template <int MT>
+int few_fp32_launch(const Product &p, cudaStream_t st) {
+  const int64_t groups = (p.N + (p.pair ? 1 : 3)) / (p.pair ? 2 : 4);
+  int share = 1;
+  while (share < 8 && groups * share < 16 * (int64_t)sm_count() && p.K[0] >= 512 * share) share *= 2;
+  const unsigned grid = (unsigned)((groups * share + 7) / 8);
+  Epilogue e = p.e;
+  e.vec = 0;  // one value a thread
+  const float *x = static_cast<const float *>(p.a[0].p), *w0 = static_cast<const float *>(p.b[0].p),
+              *w1 = static_cast<const float *>(p.b[1].p);
+  if (p.pair)
+    few_tokens_fp32_kernel<MT, true><<<grid, 256, 0, st>>>(x, p.a[0].ld, w0, p.b[0].ld, w1, p.b[1].ld, (int)p.M, (int)p.N,
+                                                           (int)p.K[0], share, e);
+  else
+    few_tokens_fp32_kernel<MT, false><<<grid, 256, 0, st>>>(x, p.a[0].ld, w0, p.b[0].ld, w1, p.b[1].ld, (int)p.M, (int)p.N,
+                                                            (int)p.K[0], share, e);
   return launch_status();
 }
 
@@ -429,12 +543,19 @@ int product(Product p, int dtype, Scratch s, int64_t &need, cudaStream_t st) {
     if (s.used > need) need = s.used;
     return s.base == nullptr ? LA_OK : few_tokens_launch(p, dtype, st);
   }
+  if (dtype == LA_F32 && few_fp32_fit(p)) {
+    if (s.used > need) need = s.used;
+    if (s.base == nullptr) return LA_OK;
+    if (p.M == 1) return few_fp32_launch<1>(p, st);
+    if (p.M == 2) return few_fp32_launch<2>(p, st);
+    return p.M <= 4 ? few_fp32_launch<4>(p, st) : few_fp32_launch<8>(p, st);
+  }
   GemmPlan plan = {0, 1};
   if (dtype == LA_F32) {
     const int64_t k = p.K[0] + (p.segments > 1 ? p.K[1] : 0);
     const int64_t tiles = (p.M + kTile - 1) / kTile * ((p.N + kTile - 1) / kTile);
-    int64_t splits = 2 * (int64_t)sm_count() / tiles;  // two CTAs per SM at least, 128 terms a split at least
-    if (splits > k / 128) splits = k / 128;
+    int64_t splits = 4 * (int64_t)sm_count() / tiles;  // up to four CTAs per SM, 64 terms a split at least
+    if (splits > k / 64) splits = k / 64;
     if (splits > 16) splits = 16;
     if (splits > 1) plan.splits = (int)splits;
   } else {
