@@ -7,8 +7,8 @@
 // a ring of TMA boxes, leaves its sums in its shared memory, and finishes a part of the tokens by adding up the sums of
 // all S through distributed shared memory, in order.  One launch, no scratch, equal calls give equal bits.
 //
-// Bound by HBM: 64 tokens through 2 x 11008 rows of 4096 (bf16) are 27.6 us at the measured copy bandwidth; 39.9 here, 49.7
-// with 256-token tiles and a second kernel for the splits of the contraction.  1 token, 4096 rows of 4096: 5.1, 10.8, 17.6.
+// Bound by HBM: 64 tokens through 2 x 11008 rows of 4096 (bf16) are 27.6 us at the measured copy bandwidth; 35.1 here, 49.7
+// with 256-token tiles and a second kernel for the splits of the contraction.  1 token, 4096 rows of 4096: 5.1, 10.5, 17.6.
 // What is left there is the launch, the first loads' way and the two cluster barriers; at 64 tokens the tokens' own boxes, which
 // every CTA reads from L2, take half of what the weights take.
 #include "linear.cuh"
@@ -29,7 +29,7 @@ constexpr uint32_t kWBytes = kRowsW * 128;
 
 template <int MT> struct Cfg {            // MT: columns, the tokens rounded up to 16, 32, 64 or 128
   static constexpr uint32_t kStage = kWBytes + MT * 128;
-  static constexpr int kStages = MT <= 16 ? 5 : (MT <= 64 ? 4 : 3);   // two CTAs fit an SM
+  static constexpr int kStages = MT <= 16 ? 4 : (MT <= 64 ? 3 : 2);   // three CTAs fit an SM
   static constexpr uint32_t kRing = kStages * kStage;
   static constexpr uint32_t kSmem = 1024 + kRing + 256;
   static constexpr uint32_t kCols = MT < 32 ? 32 : MT;
@@ -193,10 +193,10 @@ __global__ void __launch_bounds__(kThreads) few_tokens_kernel(const __grid_const
 }
 
 // The cluster's size: the largest whose clusters all fit at once (more would leave a last round with few bytes in flight).
-// How many fit is asked for once per kernel and device; the answer counts one CTA an SM, two run there (shared memory,
-// and tensor memory for three).  Measured with sizes 1 .. 8 in us: 148 tiles of 4096 31 28 31 37 35 40 39 43 (2 taken), 96 tiles
-// 25 21 28 25 24 29 28 29 (2), 64 tiles of 8192 36 28 25 24 31 29 29 29 (4), 88 tiles of 2048 13.7 12.3 12.0 15.9 16.3 (3),
-// 32 tiles of 4096 20 13 11.3 11.0 10.9 10.8 10.9 11.3 (6).
+// How many fit is asked for once per kernel and device; the answer counts one CTA an SM, three run there.  Measured with
+// sizes 1 .. 6 in us: 172 tiles of 4096 35 31.5 35 35 39 38 (2 taken), 148 tiles 32 28 33 32 31 35 (2), 96 tiles 27 21.2 20.8
+// 21.2 25 24 (4), 64 tiles of 8192 41 29 25.6 24.7 24.8 25.1 (6), 32 tiles of 4096 22 14.3 12.0 11.2 10.9 10.4 (8).  With more
+// stages and two CTAs an SM 172 tiles fitted with size 1 only, 34 us: some SMs had twice the work of others.
 template <typename T, int MT, bool PAIR>
 int launch_cfg(const FewArgs &g, int tiles, cudaStream_t st) {
   typedef Cfg<MT> C;
@@ -225,7 +225,7 @@ int launch_cfg(const FewArgs &g, int tiles, cudaStream_t st) {
   }
   if (e == cudaSuccess) {
     int size = g.stages < kMaxCluster ? g.stages : kMaxCluster;
-    while (size > 1 && 2 * fit[dev][size] < tiles) --size;
+    while (size > 1 && 3 * fit[dev][size] < tiles) --size;
     attr[0].val.clusterDim.x = (unsigned)size;
     cfg.gridDim = dim3((unsigned)(tiles * size));
     e = cudaLaunchKernelEx(&cfg, few_tokens_kernel<T, MT, PAIR>, g);
