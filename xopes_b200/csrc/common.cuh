@@ -39,6 +39,37 @@ static inline int launch_status() {
   return e == cudaSuccess ? LA_OK : LA_ERR_CUDA;
 }
 
+// Launch of a kernel that may start while the kernel before it on the stream still runs: it calls after_previous() in every
+// thread before it touches global memory (a kernel that ends without would let the one after it start too early), and
+// lets_next_start() at its beginning.  What that saves is the next kernel's launch and setup, about 1 us a kernel (10.4 to 9.6 us for a token through 4096 x 4096).
+// cluster > 0: size of the clusters of a kernel without a fixed one.
+template <typename... K, typename... A>
+static inline int launch_early(void (*kernel)(K...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, int cluster,
+                               A &&...args) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<K>(args)...);
+  if (e == cudaSuccess) return LA_OK;
+  cudaGetLastError();
+  note_cuda_error(e, "kernel launch");
+  return LA_ERR_CUDA;
+}
+#ifdef __CUDACC__
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void lets_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+#endif
+
 // While one of these lives, calls that a stream capture forbids on its thread (making a pool, a stream or an
 // event) are allowed: for what the library makes once, on first need, which may be in a capture.
 struct CaptureRelaxed {

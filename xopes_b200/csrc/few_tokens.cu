@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(kThreads) few_tokens_kernel(const __grid_const
   const int tile = blockIdx.x / size;
   const int k0 = (int)((long long)g.stages * rank / size), k1 = (int)((long long)g.stages * (rank + 1) / size);
 
+  lets_next_start();
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(full + 8 * s, 1);
@@ -104,6 +105,7 @@ __global__ void __launch_bounds__(kThreads) few_tokens_kernel(const __grid_const
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  after_previous();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(raw + (tmem_at - smem_u32(raw)));
 
   bool ok = true;
@@ -204,38 +206,32 @@ int launch_cfg(const FewArgs &g, int tiles, cudaStream_t st) {
   static int fit[64][kMaxCluster + 1];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return LA_ERR_CUDA;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C::kSmem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaError_t e = cudaSuccess;
   if (!set[dev]) {
-    e = cudaFuncSetAttribute(few_tokens_kernel<T, MT, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(few_tokens_kernel<T, MT, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)C::kSmem);
     for (int s = 1; s <= kMaxCluster && e == cudaSuccess; ++s) {
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
       attr[0].val.clusterDim.x = (unsigned)s;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3((unsigned)s);
+      cfg.blockDim = dim3(kThreads);
+      cfg.dynamicSmemBytes = C::kSmem;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
       e = cudaOccupancyMaxActiveClusters(&fit[dev][s], few_tokens_kernel<T, MT, PAIR>, &cfg);
     }
-    set[dev] = e == cudaSuccess;
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      note_cuda_error(e, "few_tokens_kernel");
+      return LA_ERR_CUDA;
+    }
+    set[dev] = true;
   }
-  if (e == cudaSuccess) {
-    int size = g.stages < kMaxCluster ? g.stages : kMaxCluster;
-    while (size > 1 && 3 * fit[dev][size] < tiles) --size;
-    attr[0].val.clusterDim.x = (unsigned)size;
-    cfg.gridDim = dim3((unsigned)(tiles * size));
-    e = cudaLaunchKernelEx(&cfg, few_tokens_kernel<T, MT, PAIR>, g);
-  }
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    note_cuda_error(e, "few_tokens_kernel");
-    return LA_ERR_CUDA;
-  }
-  return LA_OK;
+  int size = g.stages < kMaxCluster ? g.stages : kMaxCluster;
+  while (size > 1 && 3 * fit[dev][size] < tiles) --size;
+  return launch_early(few_tokens_kernel<T, MT, PAIR>, dim3((unsigned)(tiles * size)), kThreads, C::kSmem, st, size, g);
 }
 
 template <typename T, bool PAIR>

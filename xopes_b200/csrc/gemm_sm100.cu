@@ -268,6 +268,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   const int units = g.m_tiles * g.n_tiles * g.splits;
   const int first = blockIdx.x >> 1, stride = gridDim.x >> 1;
 
+  lets_next_start();
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(full + 8 * s, 1);
@@ -288,6 +289,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   __syncthreads();
   cluster_sync();
   tc_fence_after();
+  after_previous();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(raw + (tmem_at - smem_u32(raw)));
 
   if (warp == 0) {
@@ -477,8 +479,7 @@ int launch_cfg(const GemmArgs &g, int units, cudaStream_t st) {
   }
   const int pairs = sm_count() / 2;
   const int grid = 2 * (units < pairs ? units : pairs);
-  gemm_kernel<T, A_MN, B_MN, BN, PAIR><<<grid, kThreads, C::kSmem, st>>>(g);
-  return launch_status();
+  return launch_early(gemm_kernel<T, A_MN, B_MN, BN, PAIR>, dim3((unsigned)grid), kThreads, C::kSmem, st, 0, g);
 }
 
 template <typename T, int BN>

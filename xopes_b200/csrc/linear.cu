@@ -99,6 +99,8 @@ __global__ void __launch_bounds__(kSimtThreads) simt_product_kernel(const SimtAr
   const long long s0 = all * split / a.splits, s1 = all * (split + 1) / a.splits;
   float2 acc[4][4] = {}, acc2[PAIR ? 4 : 1][4] = {};  // rows 2 i and 2 i + 1, column j
   float va[8], vb[8], vb2[8];
+  lets_next_start();
+  after_previous();
   auto fetch = [&](long long s) {
     const int g = s >= a.steps[0];
     const long long k0 = (g ? s - a.steps[0] : s) * kStep;
@@ -176,6 +178,8 @@ __global__ void __launch_bounds__(256) few_tokens_fp32_kernel(const float *x, lo
                                                               int share, Epilogue e) {
   constexpr int kRows = PAIR ? 2 : 4, V = 4 * MT;
   __shared__ float part[8][32];
+  lets_next_start();
+  after_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int at = warp % share;
   const long long n0 = ((long long)blockIdx.x * 8 + warp) / share * kRows;
@@ -240,6 +244,8 @@ __global__ void __launch_bounds__(256) few_tokens_fp32_kernel(const float *x, lo
 template <typename T, bool PAIR>
 __global__ void __launch_bounds__(256) split_sum_kernel(const float *partial, int splits, long long M, int N, Epilogue e) {
   constexpr int W = 8;
+  lets_next_start();
+  after_previous();
   const int packs = (N + W - 1) / W;
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= M * packs) return;
@@ -326,6 +332,8 @@ template <typename T> struct RawKept<T, 1> {
 template <typename T, int VEC, bool PAIR>
 __global__ void __launch_bounds__(256, PAIR ? 2 : 3) act_grad_kernel(const ActGradArgs a) {
   __shared__ float part[PAIR ? 2 : 1][8][32 * VEC + 1];
+  lets_next_start();
+  after_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long n = ((long long)blockIdx.x * 32 + lane) * VEC;
   const long long r0 = (long long)blockIdx.y * a.rows, r1 = r0 + a.rows < a.M ? r0 + a.rows : a.M;
@@ -401,6 +409,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) bias_sum_kernel(const float *partial, int chunks, long long width, long long N,
                                                        void *db0, void *db1) {
   __shared__ float s[8][33];
+  lets_next_start();
+  after_previous();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const long long c = (long long)blockIdx.x * 32 + tx;
   float v = 0.f;
@@ -420,6 +430,8 @@ __global__ void __launch_bounds__(256) bias_sum_kernel(const float *partial, int
 // cores' loads want rows that start on 16 bytes; operands with other strides (odd widths) go through this copy.
 __global__ void __launch_bounds__(256) copy_rows_kernel(const uint16_t *src, long long lds, uint16_t *dst, long long ldd,
                                                         long long rows, long long cols) {
+  lets_next_start();
+  after_previous();
   const long long packs = ldd / 8, i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows * packs) return;
   const long long r = i / packs, c = (i - r * packs) * 8;
@@ -482,9 +494,8 @@ int simt_launch(const Product &p, int splits, float *partial, cudaStream_t st) {
   a.partial = partial;
   const int64_t grid = mt * a.n_tiles * splits;
   if (grid > INT32_MAX) return LA_ERR_TOO_LARGE;
-  if (p.pair) simt_product_kernel<true><<<(unsigned)grid, kSimtThreads, 0, st>>>(a);
-  else simt_product_kernel<false><<<(unsigned)grid, kSimtThreads, 0, st>>>(a);
-  return launch_status();
+  return launch_early(p.pair ? simt_product_kernel<true> : simt_product_kernel<false>, dim3((unsigned)grid), kSimtThreads, 0, st,
+                      0, a);
 }
 
 // Whether a product is few_tokens_fp32_kernel's kind, and the launch: enough warps to fill the GPU, each with 256 terms.
@@ -502,22 +513,16 @@ int few_fp32_launch(const Product &p, cudaStream_t st) {
   e.vec = 0;  // one value a thread
   const float *x = static_cast<const float *>(p.a[0].p), *w0 = static_cast<const float *>(p.b[0].p),
               *w1 = static_cast<const float *>(p.b[1].p);
-  if (p.pair)
-    few_tokens_fp32_kernel<MT, true><<<grid, 256, 0, st>>>(x, p.a[0].ld, w0, p.b[0].ld, w1, p.b[1].ld, (int)p.M, (int)p.N,
-                                                           (int)p.K[0], share, e);
-  else
-    few_tokens_fp32_kernel<MT, false><<<grid, 256, 0, st>>>(x, p.a[0].ld, w0, p.b[0].ld, w1, p.b[1].ld, (int)p.M, (int)p.N,
-                                                            (int)p.K[0], share, e);
-  return launch_status();
+  return launch_early(p.pair ? few_tokens_fp32_kernel<MT, true> : few_tokens_fp32_kernel<MT, false>, dim3(grid), 256, 0, st, 0, x,
+                      p.a[0].ld, w0, p.b[0].ld, w1, p.b[1].ld, (int)p.M, (int)p.N, (int)p.K[0], share, e);
 }
 
 template <typename T>
 int split_sum_launch(const Product &p, int splits, const float *partial, cudaStream_t st) {
   const int64_t grid = (p.M * ((p.N + 7) / 8) + 255) / 256;
   if (grid > INT32_MAX) return LA_ERR_TOO_LARGE;
-  if (p.pair) split_sum_kernel<T, true><<<(unsigned)grid, 256, 0, st>>>(partial, splits, p.M, (int)p.N, p.e);
-  else split_sum_kernel<T, false><<<(unsigned)grid, 256, 0, st>>>(partial, splits, p.M, (int)p.N, p.e);
-  return launch_status();
+  return launch_early(p.pair ? split_sum_kernel<T, true> : split_sum_kernel<T, false>, dim3((unsigned)grid), 256, 0, st, 0, partial,
+                      splits, p.M, (int)p.N, p.e);
 }
 
 // The operand as the tensor cores can read it: itself, or its copy with rows on 16-byte boundaries.
@@ -528,8 +533,8 @@ int readable(Operand &o, int64_t rows, int64_t cols, int dtype, Scratch &s, cuda
   if (s.base != nullptr) {
     const int64_t grid = (rows * (ld / 8) + 255) / 256;
     if (grid > INT32_MAX) return LA_ERR_TOO_LARGE;
-    copy_rows_kernel<<<(unsigned)grid, 256, 0, st>>>(static_cast<const uint16_t *>(o.p), o.ld, dst, ld, rows, cols);
-    const int rc = launch_status();
+    const int rc = launch_early(copy_rows_kernel, dim3((unsigned)grid), 256, 0, st, 0, static_cast<const uint16_t *>(o.p), o.ld,
+                                dst, ld, rows, cols);
     if (rc != LA_OK) return rc;
   }
   o.p = dst;
@@ -577,10 +582,9 @@ int product(Product p, int dtype, Scratch s, int64_t &need, cudaStream_t st) {
 }
 
 template <typename T, int VEC>
-void act_grad_launch(const ActGradArgs &a, bool pair, int chunks, cudaStream_t st) {
+int act_grad_launch(const ActGradArgs &a, bool pair, int chunks, cudaStream_t st) {
   const dim3 grid((unsigned)((a.N + 32 * VEC - 1) / (32 * VEC)), (unsigned)chunks);
-  if (pair) act_grad_kernel<T, VEC, true><<<grid, 256, 0, st>>>(a);
-  else act_grad_kernel<T, VEC, false><<<grid, 256, 0, st>>>(a);
+  return launch_early(pair ? act_grad_kernel<T, VEC, true> : act_grad_kernel<T, VEC, false>, grid, 256, 0, st, 0, a);
 }
 
 // chunks of rows of act_grad_kernel: one wave of the CTAs that fit, at least 8 rows (one per warp) a chunk
@@ -597,23 +601,18 @@ int act_grad(ActGradArgs a, bool pair, int chunks, void *db0, void *db1, int dty
   const int64_t per = 16 / (int64_t)dtype_size(dtype);
   const bool vec = aligned16(a.dy) && aligned16(a.z.p) && aligned16(a.dz) && a.ldy % per == 0 && a.ldz % per == 0 &&
                    a.ldd % per == 0 && a.z_up % per == 0 && a.d_up % per == 0 && a.N % per == 0;
+  int rc = LA_ERR_UNSUPPORTED;
   switch (dtype) {
-    case LA_F32: vec ? act_grad_launch<float, 4>(a, pair, chunks, st) : act_grad_launch<float, 1>(a, pair, chunks, st); break;
+    case LA_F32: rc = vec ? act_grad_launch<float, 4>(a, pair, chunks, st) : act_grad_launch<float, 1>(a, pair, chunks, st); break;
     case LA_BF16:
-      vec ? act_grad_launch<__nv_bfloat16, 8>(a, pair, chunks, st) : act_grad_launch<__nv_bfloat16, 1>(a, pair, chunks, st);
+      rc = vec ? act_grad_launch<__nv_bfloat16, 8>(a, pair, chunks, st) : act_grad_launch<__nv_bfloat16, 1>(a, pair, chunks, st);
       break;
-    case LA_F16: vec ? act_grad_launch<__half, 8>(a, pair, chunks, st) : act_grad_launch<__half, 1>(a, pair, chunks, st); break;
+    case LA_F16: rc = vec ? act_grad_launch<__half, 8>(a, pair, chunks, st) : act_grad_launch<__half, 1>(a, pair, chunks, st); break;
   }
-  int rc = launch_status();
   if (rc != LA_OK || a.partial == nullptr) return rc;
-  const int64_t width = pair ? 2 * a.N : a.N;
-  const unsigned grid = (unsigned)((width + 31) / 32);
-  switch (dtype) {
-    case LA_F32: bias_sum_kernel<float><<<grid, 256, 0, st>>>(a.partial, chunks, width, a.N, db0, db1); break;
-    case LA_BF16: bias_sum_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a.partial, chunks, width, a.N, db0, db1); break;
-    case LA_F16: bias_sum_kernel<__half><<<grid, 256, 0, st>>>(a.partial, chunks, width, a.N, db0, db1); break;
-  }
-  return launch_status();
+  const long long width = pair ? 2 * a.N : a.N;
+  auto *kernel = dtype == LA_F32 ? bias_sum_kernel<float> : (dtype == LA_BF16 ? bias_sum_kernel<__nv_bfloat16> : bias_sum_kernel<__half>);
+  return launch_early(kernel, dim3((unsigned)((width + 31) / 32)), 256, 0, st, 0, a.partial, chunks, width, a.N, db0, db1);
 }
 
 struct FwdArgs {

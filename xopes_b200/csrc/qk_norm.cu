@@ -264,8 +264,10 @@ __global__ void __launch_bounds__(kThreads) qk_norm_kernel(const __grid_constant
   const int which = blockIdx.x >= (unsigned)a.ctas[0];
   const int cta = which ? blockIdx.x - a.ctas[0] : blockIdx.x;
   const int H = a.heads[which], D = a.D, half = a.R >> 1;
+  lets_next_start();
   for (int i = threadIdx.x; i < half; i += kThreads) s_freq[i] = a.freq[i];
   __syncthreads();
+  after_previous();
   Lane<T, INTER, VEC, LPR, NP> ln;
   ln.init(a, which, inter, gl);
   float dw_lo[N] = {}, dw_hi[N] = {};
@@ -456,7 +458,9 @@ __global__ void __launch_bounds__(kThreads, VEC == 8 ? 4 : (BWD ? 5 : 6)) qk_nor
   if (threadIdx.x == 0) abort_flag = 0;
   if (lane < kDepth) ptx::mbar_init(ptx::smem_u32(&bars[warp][lane]), 1);
   ptx::fence_barrier_init();
+  lets_next_start();
   __syncthreads();
+  after_previous();
   Lane<T, INTER, VEC, LPR, 1> ln;
   ln.init(a, which, 0, gl);
   float2 dw_lo[N / 2] = {}, dw_hi[N / 2] = {};
@@ -600,6 +604,8 @@ template <typename T>
 __global__ void __launch_bounds__(1024) qk_norm_dw_kernel(const float *pq, const float *pk, int rows_q, int rows_k, int D,
                                                           void *dwq, void *dwk, int w16) {
   __shared__ float s[32][33];
+  lets_next_start();
+  after_previous();
   const int k = blockIdx.y, rows = k ? rows_k : rows_q;
   const float *p = k ? pk : pq;
   void *dw = k ? dwk : dwq;
@@ -669,8 +675,7 @@ int launch_cfg(QkArgs &a, int inter, const bool (&mine)[2], cudaStream_t st) {
     a.items[k] = mine[k] ? groups * a.chunks[k] : 0;
   }
   share_ctas(a, (long long)sms * resident);
-  qk_norm_kernel<T, BWD, INTER, VEC, LPR, NP><<<a.ctas[0] + a.ctas[1], kThreads, 0, st>>>(a, inter);
-  return launch_status();
+  return launch_early(qk_norm_kernel<T, BWD, INTER, VEC, LPR, NP>, dim3(a.ctas[0] + a.ctas[1]), kThreads, 0, st, 0, a, inter);
 }
 
 template <typename T, bool BWD, bool INTER, int VEC, int LPR>
@@ -701,8 +706,8 @@ int launch_stream(QkArgs &a, const bool (&mine)[2], cudaStream_t st) {
     a.items[k] = mine[k] ? a.T : 0;
   }
   share_ctas(a, (long long)sms * resident[dev]);
-  qk_norm_stream_kernel<T, BWD, INTER, VEC, LPR><<<a.ctas[0] + a.ctas[1], kThreads, kSmem, st>>>(a, status_word_ptr());
-  return launch_status();
+  return launch_early(qk_norm_stream_kernel<T, BWD, INTER, VEC, LPR>, dim3(a.ctas[0] + a.ctas[1]), kThreads, kSmem, st, 0, a,
+                      status_word_ptr());
 }
 
 // Streamed: tensors whose heads lie next to each other and fill a warp's rows, from 2^20 elements on.  Measured, forward /
@@ -877,13 +882,9 @@ int la_qk_norm_rope_bwd(const void *q, int64_t q_sb, int64_t q_sn, int64_t q_sh,
   const int rc2 = dispatch<true>(a, dtype, interleaved != 0, st);
   if (rc2 != LA_OK || !want_dw) return rc2;
   const dim3 grid((unsigned)((D + 31) / 32), 2);
-  if (dtype == LA_F16)
-    qk_norm_dw_kernel<__half><<<grid, 1024, 0, st>>>(a.partial[0], a.partial[1], a.ctas[0], a.ctas[1], (int)D, dq_weight,
-                                                     dk_weight, a.w16);
-  else
-    qk_norm_dw_kernel<__nv_bfloat16><<<grid, 1024, 0, st>>>(a.partial[0], a.partial[1], a.ctas[0], a.ctas[1], (int)D,
-                                                            dq_weight, dk_weight, a.w16 && dtype != LA_F32);
-  return launch_status();
+  const int w16 = a.w16 && dtype != LA_F32;
+  return launch_early(dtype == LA_F16 ? qk_norm_dw_kernel<__half> : qk_norm_dw_kernel<__nv_bfloat16>, grid, 1024, 0, st, 0,
+                      a.partial[0], a.partial[1], a.ctas[0], a.ctas[1], (int)D, dq_weight, dk_weight, w16);
 }
 
 }  // extern "C"
