@@ -49,74 +49,108 @@ struct SimtArgs {
   Epilogue e;
 };
 
-constexpr int kTile = 64, kStep = 16, kPitch = kTile + 4, kSimtThreads = 128;
+constexpr int kStep = 16;
+template <int TILE> constexpr int simt_threads() { return TILE == 128 ? 256 : 128; }
 
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 
-// eight elements of a 64 x 16 operand tile for this thread, two quads: along the contraction, or along the rows (mn_major)
-__device__ __forceinline__ void simt_fetch(const Operand &o, int vec, long long r0, long long R, long long k0, long long K,
-                                           float (&v)[8]) {
-  const int t = threadIdx.x;
-  const float *p = static_cast<const float *>(o.p);
+// A thread's share of the TILE x 16 tiles of an operand, step after step: two quads, along the contraction or along the rows
+// (mn_major).
+template <int TILE> struct SimtLoad {
+  const float *p[2];
+  long long step;
+  int left;  // along the contraction: bits of the rows that exist; along the rows: rows that exist from the quad's first on
+  bool mn, vec;
+  __device__ __forceinline__ void init(const Operand &o, int vec_, long long r0, long long R, long long k0) {
+    const int t = threadIdx.x;
+    const float *base = static_cast<const float *>(o.p);
+    mn = o.mn_major;
+    vec = vec_;
+    left = 0;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float (&q)[4] = reinterpret_cast<float (&)[4]>(v[4 * i]);
-    q[0] = q[1] = q[2] = q[3] = 0.f;
-    if (!o.mn_major) {
-      const long long r = r0 + (t >> 2) + 32 * i, k = k0 + (t & 3) * 4;
-      if (r < R) load_row<float, 4>(p + r * o.ld + k, vec, (int)(K - k < 4 ? K - k : 4), q);
-    } else {
-      const long long k = k0 + (t >> 4) + 8 * i, r = r0 + (t & 15) * 4;
-      if (k < K) load_row<float, 4>(p + k * o.ld + r, vec, (int)(R - r < 4 ? R - r : 4), q);
+    for (int i = 0; i < 2; ++i) {
+      if (!mn) {
+        const long long r = r0 + (t >> 2) + TILE / 2 * i;
+        p[i] = base + r * o.ld + k0 + (t & 3) * 4;
+        left |= (r < R) << i;
+      } else {
+        const long long r = r0 + t % (TILE / 4) * 4;
+        p[i] = base + (k0 + t / (TILE / 4) + 8 * i) * o.ld + r;
+        left = R - r < 4 ? (int)(R - r) : 4;
+      }
+    }
+    step = mn ? kStep * o.ld : kStep;
+  }
+  // the next step, of which k_left terms exist
+  __device__ __forceinline__ void fetch(int k_left, float (&v)[8]) {
+    const int t = threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float (&q)[4] = reinterpret_cast<float (&)[4]>(v[4 * i]);
+      const int exist = !mn ? (left >> i & 1 ? k_left - (t & 3) * 4 : 0) : (t / (TILE / 4) + 8 * i < k_left ? left : 0);
+      load_row<float, 4>(p[i], vec, exist, q);
+      p[i] += step;
     }
   }
-}
-__device__ __forceinline__ void simt_put(const Operand &o, float (*s)[kPitch], const float (&v)[8]) {
+};
+template <int TILE>
+__device__ __forceinline__ void simt_put(bool mn, float (*s)[TILE + 4], const float (&v)[8]) {
   const int t = threadIdx.x;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    if (!o.mn_major) {
+    if (!mn) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[(t & 3) * 4 + j][(t >> 2) + 32 * i] = v[4 * i + j];
+      for (int j = 0; j < 4; ++j) s[(t & 3) * 4 + j][(t >> 2) + TILE / 2 * i] = v[4 * i + j];
     } else {
-      *reinterpret_cast<float4 *>(&s[(t >> 4) + 8 * i][(t & 15) * 4]) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      *reinterpret_cast<float4 *>(&s[t / (TILE / 4) + 8 * i][t % (TILE / 4) * 4]) =
+          make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
     }
   }
 }
 
-// One 64 x 64 tile (of one split) per CTA of 128 threads, 8 x 4 results a thread, packed over pairs of rows; the next step's
-// operands are in registers while the current step's are multiplied.  514 x 512 x 512 17 us with the sum of the splits,
-// 2048 x 2048 x 2048 436 us (39 TFLOP/s; fp32 units and the instructions beside the products bound it; elements of B kept twice
-// in shared memory, to save the doubling, made shared memory the bound: 860 us).
-template <bool PAIR>
-__global__ void __launch_bounds__(kSimtThreads) simt_product_kernel(const SimtArgs a) {
-  __shared__ __align__(16) float sa[2][kStep][kPitch], sb[2][PAIR ? 2 : 1][kStep][kPitch];
+// One TILE x TILE tile (of one split) per CTA, 8 x 4 results a thread (TILE 64, 128 threads) or 8 x 8 (TILE 128, 256 threads),
+// packed over pairs of rows; the next step's operands are in registers while the current step's are multiplied.
+// 2048 x 2048 x 2048 426 us (40 TFLOP/s; the instructions beside the products and shared memory bound it; elements of B kept
+// twice in shared memory, to save doubling them in registers, 860 us), 514 x 512 x 512 17.5 us with the sum of the splits.
+template <int TILE, bool PAIR>
+__global__ void __launch_bounds__(simt_threads<TILE>(), TILE == 128 ? 2 : (PAIR ? 3 : 5)) simt_product_kernel(const SimtArgs a) {
+  constexpr int TN = TILE / 16;  // columns a thread: 4 from tx * 4 on, and for TILE 128 4 from 64 + tx * 4 on
+  __shared__ __align__(16) float sa[2][kStep][TILE + 4], sb[2][PAIR ? 2 : 1][kStep][TILE + 4];
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const long long tile = blockIdx.x / a.splits;
   const int split = (int)(blockIdx.x - tile * a.splits);
-  const long long m0 = tile / a.n_tiles * kTile, n0 = tile % a.n_tiles * kTile;
+  const long long m0 = tile / a.n_tiles * TILE, n0 = tile % a.n_tiles * TILE;
   const long long all = a.steps[0] + a.steps[1];
   const long long s0 = all * split / a.splits, s1 = all * (split + 1) / a.splits;
-  float2 acc[4][4] = {}, acc2[PAIR ? 4 : 1][4] = {};  // rows 2 i and 2 i + 1, column j
+  float2 acc[4][TN] = {}, acc2[PAIR ? 4 : 1][TN] = {};  // rows 2 i and 2 i + 1, column j
   float va[8], vb[8], vb2[8];
   lets_next_start();
   after_previous();
+  SimtLoad<TILE> la, lb, lb2;
+  long long k_left = 0;  // terms of the segment from the next step on
   auto fetch = [&](long long s) {
-    const int g = s >= a.steps[0];
-    const long long k0 = (g ? s - a.steps[0] : s) * kStep;
-    simt_fetch(a.a[g], a.vec_a[g], m0, a.M, k0, a.K[g], va);
-    simt_fetch(a.b[g], a.vec_b[g], n0, a.N, k0, a.K[g], vb);
-    if (PAIR) simt_fetch(a.b[1], a.vec_b[1], n0, a.N, k0, a.K[0], vb2);
+    if (s == s0 || s == a.steps[0]) {  // the first step here, or of the second segment
+      const int g = s >= a.steps[0];
+      const long long k0 = (g ? s - a.steps[0] : s) * kStep;
+      la.init(a.a[g], a.vec_a[g], m0, a.M, k0);
+      lb.init(a.b[g], a.vec_b[g], n0, a.N, k0);
+      if (PAIR) lb2.init(a.b[1], a.vec_b[1], n0, a.N, k0);
+      k_left = a.K[g] - k0;
+    }
+    const int some = k_left < kStep ? (int)k_left : kStep;
+    la.fetch(some, va);
+    lb.fetch(some, vb);
+    if (PAIR) lb2.fetch(some, vb2);
+    k_left -= kStep;
   };
-  auto put = [&](long long s, int at) {
-    const int g = s >= a.steps[0];
-    simt_put(a.a[g], sa[at], va);
-    simt_put(a.b[g], sb[at][0], vb);
-    if (PAIR) simt_put(a.b[1], sb[at][PAIR ? 1 : 0], vb2);
+  auto put = [&](int at) {  // both operands of a step lie the same way in both segments
+    simt_put<TILE>(la.mn, sa[at], va);
+    simt_put<TILE>(lb.mn, sb[at][0], vb);
+    if (PAIR) simt_put<TILE>(lb2.mn, sb[at][PAIR ? 1 : 0], vb2);
   };
   if (s0 < s1) {
     fetch(s0);
-    put(s0, 0);
+    put(0);
   }
   __syncthreads();
   for (long long s = s0; s < s1; ++s) {
@@ -125,45 +159,51 @@ __global__ void __launch_bounds__(kSimtThreads) simt_product_kernel(const SimtAr
 #pragma unroll
     for (int k = 0; k < kStep; ++k) {
       float2 x[4];
-      float y[4];
+      float y[TN];
       *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(&sa[at][k][ty * 8]);
       *reinterpret_cast<float4 *>(x + 2) = *reinterpret_cast<const float4 *>(&sa[at][k][ty * 8 + 4]);
-      *reinterpret_cast<float4 *>(y) = *reinterpret_cast<const float4 *>(&sb[at][0][k][tx * 4]);
+#pragma unroll
+      for (int j = 0; j < TN; j += 4)
+        *reinterpret_cast<float4 *>(y + j) = *reinterpret_cast<const float4 *>(&sb[at][0][k][tx * 4 + 16 * j]);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fma2(x[i], make_float2(y[j], y[j]), acc[i][j]);
+        for (int j = 0; j < TN; ++j) acc[i][j] = fma2(x[i], make_float2(y[j], y[j]), acc[i][j]);
       if (PAIR) {
-        *reinterpret_cast<float4 *>(y) = *reinterpret_cast<const float4 *>(&sb[at][PAIR ? 1 : 0][k][tx * 4]);
+#pragma unroll
+        for (int j = 0; j < TN; j += 4)
+          *reinterpret_cast<float4 *>(y + j) = *reinterpret_cast<const float4 *>(&sb[at][PAIR ? 1 : 0][k][tx * 4 + 16 * j]);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc2[PAIR ? i : 0][j] = fma2(x[i], make_float2(y[j], y[j]), acc2[PAIR ? i : 0][j]);
+          for (int j = 0; j < TN; ++j) acc2[PAIR ? i : 0][j] = fma2(x[i], make_float2(y[j], y[j]), acc2[PAIR ? i : 0][j]);
       }
     }
-    if (s + 1 < s1) put(s + 1, at ^ 1);
+    if (s + 1 < s1) put(at ^ 1);
     __syncthreads();
   }
-  const long long n = n0 + tx * 4;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const long long m = m0 + ty * 8 + i;
-    if (m >= a.M || n >= a.N) continue;
-    float p[4], q[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      p[j] = i % 2 ? acc[i / 2][j].y : acc[i / 2][j].x;
-      q[j] = i % 2 ? acc2[PAIR ? i / 2 : 0][j].y : acc2[PAIR ? i / 2 : 0][j].x;
-    }
-    if (a.partial != nullptr) {
-      float *o = a.partial + ((long long)split * (PAIR ? 2 : 1) * a.M + m) * a.N + n;
-      const int left = (int)(a.N - n < 4 ? a.N - n : 4);
-      store_row<float, 4>(o, a.N % 4 == 0, left, p);
-      if (PAIR) store_row<float, 4>(o + a.M * a.N, a.N % 4 == 0, left, q);
-    } else if (PAIR) {
-      finish_pair<float, 4>(a.e, m, (int)n, (int)a.N, p, q);
-    } else {
-      finish_one<float, 4>(a.e, m, (int)n, (int)a.N, p);
+    for (int h = 0; h < TN / 4; ++h) {
+      const long long m = m0 + ty * 8 + i, n = n0 + tx * 4 + 64 * h;
+      if (m >= a.M || n >= a.N) continue;
+      float p[4], q[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        p[j] = i % 2 ? acc[i / 2][4 * h + j].y : acc[i / 2][4 * h + j].x;
+        q[j] = i % 2 ? acc2[PAIR ? i / 2 : 0][4 * h + j].y : acc2[PAIR ? i / 2 : 0][4 * h + j].x;
+      }
+      if (a.partial != nullptr) {
+        float *o = a.partial + ((long long)split * (PAIR ? 2 : 1) * a.M + m) * a.N + n;
+        const int left = (int)(a.N - n < 4 ? a.N - n : 4);
+        store_row<float, 4>(o, a.N % 4 == 0, left, p);
+        if (PAIR) store_row<float, 4>(o + a.M * a.N, a.N % 4 == 0, left, q);
+      } else if (PAIR) {
+        finish_pair<float, 4>(a.e, m, (int)n, (int)a.N, p, q);
+      } else {
+        finish_one<float, 4>(a.e, m, (int)n, (int)a.N, p);
+      }
     }
   }
 }
@@ -478,7 +518,31 @@ int epilogue_vec(const Epilogue &e, int dtype) {
          aligned16(e.save.p) && e.ldr % per == 0 && e.ldo % per == 0 && e.lds % per == 0 && e.save_up % per == 0;
 }
 
-int simt_launch(const Product &p, int splits, float *partial, cudaStream_t st) {
+// Tile and splits of an fp32 product.  Tiles of 128 where the result is wider than 64 both ways and they and their splits
+// fill the GPU, else of 64; splits for two (tiles of 128) or four CTAs an SM, of at least 256 or 64 terms.  With tiles of 64 /
+// of 128: 1024 x 1024 x 1024 73 / 63 us, 700 x 2000 x 3008 250 / 207, 16 x 4096 x 4096 65 / 101.
+struct SimtPlan {
+  int tile, splits;
+};
+SimtPlan simt_plan(const Product &p) {
+  const int64_t k = p.K[0] + (p.segments > 1 ? p.K[1] : 0), sms = sm_count();
+  auto plan = [&](int tile, int64_t per_sm, int64_t terms) {
+    const int64_t tiles = (p.M + tile - 1) / tile * ((p.N + tile - 1) / tile);
+    int64_t splits = per_sm * sms / tiles;
+    if (splits > k / terms) splits = k / terms;
+    if (splits > 16) splits = 16;
+    if (splits < 1) splits = 1;
+    return SimtPlan{tile, (int)splits};
+  };
+  if (!p.pair && p.M > 64 && p.N > 64) {
+    const SimtPlan big = plan(128, 2, 256);
+    const int64_t tiles = (p.M + 127) / 128 * ((p.N + 127) / 128);
+    if (tiles * big.splits >= sms) return big;
+  }
+  return plan(64, 4, 64);
+}
+
+int simt_launch(const Product &p, const SimtPlan &plan, float *partial, cudaStream_t st) {
   SimtArgs a = {};
   a.M = p.M; a.N = p.N; a.e = p.e;
   for (int s = 0; s < 2; ++s) {
@@ -488,14 +552,16 @@ int simt_launch(const Product &p, int splits, float *partial, cudaStream_t st) {
     a.vec_a[s] = aligned16(p.a[s].p) && p.a[s].ld % 4 == 0;
     a.vec_b[s] = aligned16(p.b[s].p) && p.b[s].ld % 4 == 0;
   }
-  const int64_t mt = (p.M + kTile - 1) / kTile;
-  a.n_tiles = (int)((p.N + kTile - 1) / kTile);
-  a.splits = splits;
+  const int64_t mt = (p.M + plan.tile - 1) / plan.tile;
+  a.n_tiles = (int)((p.N + plan.tile - 1) / plan.tile);
+  a.splits = plan.splits;
   a.partial = partial;
-  const int64_t grid = mt * a.n_tiles * splits;
+  const int64_t grid = mt * a.n_tiles * plan.splits;
   if (grid > INT32_MAX) return LA_ERR_TOO_LARGE;
-  return launch_early(p.pair ? simt_product_kernel<true> : simt_product_kernel<false>, dim3((unsigned)grid), kSimtThreads, 0, st,
-                      0, a);
+  if (plan.tile == 128)
+    return launch_early(simt_product_kernel<128, false>, dim3((unsigned)grid), simt_threads<128>(), 0, st, 0, a);
+  return launch_early(p.pair ? simt_product_kernel<64, true> : simt_product_kernel<64, false>, dim3((unsigned)grid),
+                      simt_threads<64>(), 0, st, 0, a);
 }
 
 // Whether a product is few_tokens_fp32_kernel's kind, and the launch: enough warps to fill the GPU, each with 256 terms.
@@ -556,13 +622,10 @@ int product(Product p, int dtype, Scratch s, int64_t &need, cudaStream_t st) {
     return p.M <= 4 ? few_fp32_launch<4>(p, st) : few_fp32_launch<8>(p, st);
   }
   GemmPlan plan = {0, 1};
+  SimtPlan simt = {0, 1};
   if (dtype == LA_F32) {
-    const int64_t k = p.K[0] + (p.segments > 1 ? p.K[1] : 0);
-    const int64_t tiles = (p.M + kTile - 1) / kTile * ((p.N + kTile - 1) / kTile);
-    int64_t splits = 4 * (int64_t)sm_count() / tiles;  // up to four CTAs per SM, 64 terms a split at least
-    if (splits > k / 64) splits = k / 64;
-    if (splits > 16) splits = 16;
-    if (splits > 1) plan.splits = (int)splits;
+    simt = simt_plan(p);
+    plan.splits = simt.splits;
   } else {
     plan = gemm_plan(p.M, p.N, p.K[0], p.segments > 1 ? p.K[1] : 0, p.pair != 0);
   }
@@ -571,7 +634,7 @@ int product(Product p, int dtype, Scratch s, int64_t &need, cudaStream_t st) {
   if (s.used > need) need = s.used;
   if (s.base == nullptr) return LA_OK;
   p.e.vec = epilogue_vec(p.e, dtype);
-  const int rc = dtype == LA_F32 ? simt_launch(p, plan.splits, partial, st) : gemm_launch(p, plan, partial, dtype, st);
+  const int rc = dtype == LA_F32 ? simt_launch(p, simt, partial, st) : gemm_launch(p, plan, partial, dtype, st);
   if (rc != LA_OK || partial == nullptr) return rc;
   switch (dtype) {
     case LA_F32: return split_sum_launch<float>(p, plan.splits, partial, st);
