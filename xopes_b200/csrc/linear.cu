@@ -52,8 +52,6 @@ struct SimtArgs {
 constexpr int kStep = 16;
 template <int TILE> constexpr int simt_threads() { return TILE == 128 ? 256 : 128; }
 
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
-
 // A thread's share of the TILE x 16 tiles of an operand, step after step: two quads, along the contraction or along the rows
 // (mn_major).
 template <int TILE> struct SimtLoad {
@@ -382,24 +380,31 @@ __global__ void __launch_bounds__(256, PAIR ? 2 : 3) act_grad_kernel(const ActGr
   if (n < a.N) {  // N is a multiple of VEC
     RawRow<T, VEC> dy[2];
     RawKept<T, VEC> z[2], u[2];
-    auto fetch = [&](long long m, int i) {
-      dy[i].load(static_cast<const T *>(a.dy) + m * a.ldy + n);
-      if (kept) z[i].load(a.z, m * a.ldz + n);
-      if (PAIR) u[i].load(a.z, m * a.ldz + a.z_up + n);
-    };
     long long m = r0 + warp;
-    if (m < r1) fetch(m, 0);
-    if (m + 8 < r1) fetch(m + 8, 1);
-    for (; m < r1; m += 16) {
+    // the next row to load and to store; rows of a warp are 8 apart
+    const T *dyp = static_cast<const T *>(a.dy) + m * a.ldy + n;
+    long long zo = m * a.ldz + n;
+    T *op = a.dz == nullptr ? nullptr : static_cast<T *>(a.dz) + m * a.ldd + n;
+    const long long dys = 8 * a.ldy, zs = 8 * a.ldz, os = 8 * a.ldd;
+    auto fetch = [&](int i) {
+      dy[i].load(dyp);
+      if (kept) z[i].load(a.z, zo);
+      if (PAIR) u[i].load(a.z, zo + a.z_up);
+      dyp += dys;
+      zo += zs;
+    };
+    const int rows = m < r1 ? (int)((r1 - m + 7) / 8) : 0;  // of this warp
+    if (rows > 0) fetch(0);
+    if (rows > 1) fetch(1);
+    for (int row = 0; row < rows; row += 2) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const long long mi = m + 8 * i;
-        if (mi >= r1) break;
+        if (row + i >= rows) break;
         float d[VEC], p[VEC], q[VEC], g[VEC];
         dy[i].get(d);
         if (kept) z[i].get(p);
         if (PAIR) u[i].get(q);
-        if (mi + 16 < r1) fetch(mi + 16, i);
+        if (row + i + 2 < rows) fetch(i);
         if (kept) {
           activate_grad<T, VEC>(p, g, a.act);
 #pragma unroll
@@ -414,10 +419,10 @@ __global__ void __launch_bounds__(256, PAIR ? 2 : 3) act_grad_kernel(const ActGr
         }
 #pragma unroll
         for (int j = 0; j < VEC; ++j) s0[j] += d[j];
-        if (a.dz != nullptr) {
-          T *o = static_cast<T *>(a.dz) + mi * a.ldd + n;
-          store_row<T, VEC>(o, VEC > 1, VEC, d);
-          if (PAIR) store_row<T, VEC>(o + a.d_up, VEC > 1, VEC, p);
+        if (op != nullptr) {
+          store_row<T, VEC>(op, VEC > 1, VEC, d);
+          if (PAIR) store_row<T, VEC>(op + a.d_up, VEC > 1, VEC, p);
+          op += os;
         }
       }
     }

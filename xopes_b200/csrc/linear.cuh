@@ -11,28 +11,38 @@ namespace lin {
 
 enum { kActNone = 0, kActRelu = 1, kActSigmoid = 2, kActSilu = 3, kActGelu = 4 };
 
-// e^x: 2 ulp for fp32 results; the fast form (2 + 1.2 |x| ulp) where the result is rounded to 16 bits
-template <typename T> __device__ __forceinline__ float exp_of(float x) { return __expf(x); }
-template <> __device__ __forceinline__ float exp_of<float>(float x) { return expf(x); }
-template <typename T> __device__ __forceinline__ float inverse_of(float x) { return __fdividef(1.f, x); }
-template <> __device__ __forceinline__ float inverse_of<float>(float x) { return 1.f / x; }
-// 1 / (1 + e^-z); the fast quotient returns 0 for divisors above 2^126, which is what the sigmoid is there
-template <typename T> __device__ __forceinline__ float sigmoid_of(float z) { return inverse_of<T>(1.f + exp_of<T>(-z)); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float ex2(float x) {  // 2^x, one instruction
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float2 ex2(float2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
+// 1 / x; 0 for x above 2^126
+__device__ __forceinline__ float2 inverse2(float2 x) { return make_float2(__fdividef(1.f, x.x), __fdividef(1.f, x.y)); }
+constexpr float kLog2e = 1.4426950408889634f;
 
-// Phi(z), the normal distribution's integral, with e = e^(-z^2 / 2).  fp32: by erf.  Where the result is rounded to 16
-// bits: Abramowitz and Stegun 7.1.26, 1 - (a1 t + .. + a5 t^5) e with t = 1 / (1 + p |z| / sqrt 2), absolute error
-// 1.5e-7, which shares its exponential with the density (erff took 2/3 of the derivative pass's instructions).
-template <typename T> __device__ __forceinline__ float normal_cdf(float z, float &e) {
-  e = exp_of<T>(-0.5f * z * z);
-  const float t = __fdividef(1.f, fmaf(0.23164189f, fabsf(z), 1.f));
-  const float q = t * e * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f),
-                               0.127414796f);
-  return z < 0.f ? q : 1.f - q;
+// Sigmoid and the normal distribution's integral in two forms.  fp32 results: by expf (2 ulp) and erff, one value at a time.
+// Results that are rounded to 16 bits: by 2^x and 1 / x of the special function unit, two values in packed arithmetic.
+
+// 1 / (1 + e^-z)
+__device__ __forceinline__ float2 sigmoid2(float2 z) { return inverse2(add2(both(1.f), ex2(mul2(z, both(-kLog2e))))); }
+__device__ __forceinline__ float sigmoid_exact(float z) { return 1.f / (1.f + expf(-z)); }
+// Phi(z), and e = e^(-z^2 / 2).  Abramowitz and Stegun 7.1.26, 1 - (a1 t + .. + a5 t^5) e with t = 1 / (1 + p |z| / sqrt 2),
+// absolute error 1.5e-7, which shares its exponential with the density (erff took 2/3 of the derivative pass's instructions).
+__device__ __forceinline__ float2 normal_cdf2(float2 z, float2 &e) {
+  e = ex2(mul2(mul2(z, z), both(-0.5f * kLog2e)));
+  const float2 t = inverse2(fma2(both(0.23164189f), make_float2(fabsf(z.x), fabsf(z.y)), both(1.f)));
+  float2 q = fma2(t, both(0.5307027145f), both(-0.7265760135f));
+  q = fma2(t, q, both(0.7107068705f));
+  q = fma2(t, q, both(-0.142248368f));
+  q = mul2(mul2(t, e), fma2(t, q, both(0.127414796f)));
+  return make_float2(z.x < 0.f ? q.x : 1.f - q.x, z.y < 0.f ? q.y : 1.f - q.y);
 }
-template <> __device__ __forceinline__ float normal_cdf<float>(float z, float &e) {
-  e = expf(-0.5f * z * z);
-  return 0.5f + 0.5f * erff(z * 0.70710678118654752f);
-}
+__device__ __forceinline__ float normal_cdf_exact(float z) { return 0.5f + 0.5f * erff(z * 0.70710678118654752f); }
 
 // z[j] = act(z[j]); the kind is the same for the whole launch, so the choice is a branch around a row's loop
 template <typename T, int W>
@@ -40,17 +50,33 @@ __device__ __forceinline__ void activate(float (&z)[W], int kind) {
   if (kind == kActRelu) {
 #pragma unroll
     for (int j = 0; j < W; ++j) z[j] = z[j] > 0.f || z[j] != z[j] ? z[j] : 0.f;
-  } else if (kind == kActSigmoid) {
+    return;
+  }
+  if constexpr (sizeof(T) == 2 && W % 2 == 0) {
+    float2 (&v)[W / 2] = reinterpret_cast<float2 (&)[W / 2]>(z);
+    if (kind == kActSigmoid) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) z[j] = sigmoid_of<T>(z[j]);
-  } else if (kind == kActSilu) {
+      for (int j = 0; j < W / 2; ++j) v[j] = sigmoid2(v[j]);
+    } else if (kind == kActSilu) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) z[j] *= sigmoid_of<T>(z[j]);
-  } else if (kind == kActGelu) {
+      for (int j = 0; j < W / 2; ++j) v[j] = mul2(v[j], sigmoid2(v[j]));
+    } else if (kind == kActGelu) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      float e;
-      z[j] *= normal_cdf<T>(z[j], e);
+      for (int j = 0; j < W / 2; ++j) {
+        float2 e;
+        v[j] = mul2(v[j], normal_cdf2(v[j], e));
+      }
+    }
+  } else {
+    if (kind == kActSigmoid) {
+#pragma unroll
+      for (int j = 0; j < W; ++j) z[j] = sigmoid_exact(z[j]);
+    } else if (kind == kActSilu) {
+#pragma unroll
+      for (int j = 0; j < W; ++j) z[j] *= sigmoid_exact(z[j]);
+    } else if (kind == kActGelu) {
+#pragma unroll
+      for (int j = 0; j < W; ++j) z[j] *= normal_cdf_exact(z[j]);
     }
   }
 }
@@ -58,36 +84,58 @@ __device__ __forceinline__ void activate(float (&z)[W], int kind) {
 // z[j] = act(z[j]) and d[j] = act'(z[j])
 template <typename T, int W>
 __device__ __forceinline__ void activate_grad(float (&z)[W], float (&d)[W], int kind) {
+  constexpr float kDensity = 0.3989422804014327f;  // 1 / sqrt(2 pi)
   if (kind == kActRelu) {
 #pragma unroll
     for (int j = 0; j < W; ++j) {
       d[j] = z[j] > 0.f ? 1.f : 0.f;
       z[j] = z[j] > 0.f || z[j] != z[j] ? z[j] : 0.f;
     }
-  } else if (kind == kActSigmoid) {
+    return;
+  }
+  if (kind == kActNone) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      z[j] = sigmoid_of<T>(z[j]);
-      d[j] = z[j] * (1.f - z[j]);
-    }
-  } else if (kind == kActSilu) {
+    for (int j = 0; j < W; ++j) d[j] = 1.f;
+    return;
+  }
+  if constexpr (sizeof(T) == 2 && W % 2 == 0) {
+    float2 (&v)[W / 2] = reinterpret_cast<float2 (&)[W / 2]>(z), (&g)[W / 2] = reinterpret_cast<float2 (&)[W / 2]>(d);
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const float s = sigmoid_of<T>(z[j]);
-      d[j] = s * (1.f + z[j] * (1.f - s));
-      z[j] *= s;
-    }
-  } else if (kind == kActGelu) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      float e;
-      const float cdf = normal_cdf<T>(z[j], e);
-      d[j] = cdf + z[j] * 0.3989422804014327f * e;
-      z[j] *= cdf;
+    for (int j = 0; j < W / 2; ++j) {
+      if (kind == kActGelu) {
+        float2 e;
+        const float2 cdf = normal_cdf2(v[j], e);
+        g[j] = fma2(mul2(v[j], both(kDensity)), e, cdf);
+        v[j] = mul2(v[j], cdf);
+      } else {
+        const float2 s = sigmoid2(v[j]), rest = fma2(s, both(-1.f), both(1.f));
+        if (kind == kActSilu) {
+          v[j] = mul2(v[j], s);
+          g[j] = fma2(v[j], rest, s);
+        } else {
+          v[j] = s;
+          g[j] = mul2(s, rest);
+        }
+      }
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < W; ++j) d[j] = 1.f;
+    for (int j = 0; j < W; ++j) {
+      if (kind == kActGelu) {
+        const float cdf = normal_cdf_exact(z[j]);
+        d[j] = cdf + z[j] * kDensity * expf(-0.5f * z[j] * z[j]);
+        z[j] *= cdf;
+      } else {
+        const float s = sigmoid_exact(z[j]);
+        if (kind == kActSilu) {
+          d[j] = s * (1.f + z[j] * (1.f - s));
+          z[j] *= s;
+        } else {
+          z[j] = s;
+          d[j] = s * (1.f - s);
+        }
+      }
+    }
   }
 }
 
