@@ -157,3 +157,48 @@ def test_tensors_of_another_stream():
             outs.append(block(x, w, ld, 4, 64)[0])
         torch.cuda.synchronize()
     assert all(torch.equal(ref, o) for o in outs)
+
+
+FIRST = """
+import torch
+from xopes_b200.linear import gated_linear_fn, linear_fn
+from xopes_b200.qk_norm import qk_norm_rope_fn
+def rand(*s):
+    return torch.randn(*s, device="cuda").mul(0.1).to(torch.%s)
+torch.manual_seed(0)
+m = %d
+x, w, v, b, q = rand(m, 256), rand(320, 256), rand(320, 256), rand(320), rand(1, m, 16, 128)
+def call():
+    return [linear_fn(x, w, b, act="gelu"), gated_linear_fn(x, w, v, b), *qk_norm_rope_fn(q, q)]
+torch.cuda.synchronize()
+with torch.no_grad():
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    graph.replay()
+    ref = call()
+    torch.cuda.synchronize()
+for o, r in zip(out, ref):
+    assert torch.isfinite(o.float()).all() and torch.equal(o, r)
+"""
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("m", [3, 600])
+def test_first_use_under_capture(m, dtype):
+    """What the kernels need once per device is found inside a capture too."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", FIRST % (dtype, m)], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]
+
+
+def test_second_derivatives_are_refused():
+    from xopes_b200.linear import gated_linear_fn, linear_fn
+    from xopes_b200.qk_norm import qk_norm_rope_fn
+    x, w = (torch.randn(8, 8, device="cuda").requires_grad_() for _ in range(2))
+    for y in (linear_fn(x, w), gated_linear_fn(x, w, w), qk_norm_rope_fn(x.view(1, 8, 1, 8), x.view(1, 8, 1, 8))[0]):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)

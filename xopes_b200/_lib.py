@@ -148,6 +148,13 @@ def require_cuda(*tensors):
             raise RuntimeError("xopes_b200 operators run on CUDA tensors only (no CPU fallback)")
 
 
+def once_differentiable():
+    """For backward passes: they are kernels that autograd cannot see through, so a graph of them (create_graph=True)
+    would give wrong second derivatives."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("this operator is differentiable once: create_graph=True is not supported")
+
+
 def check(rc: int, what: str):
     if rc != 0:
         lib = load()

@@ -13,8 +13,10 @@ char *last_cuda_error_buf() {
   return buf;
 }
 
+static int *g_status_ptrs[64] = {nullptr};
+
 int *status_word_ptr() {
-  static int *ptrs[64] = {nullptr};
+  int **ptrs = g_status_ptrs;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
   if (ptrs[dev] == nullptr) {
@@ -23,6 +25,18 @@ int *status_word_ptr() {
     ptrs[dev] = static_cast<int *>(p);
   }
   return ptrs[dev];
+}
+
+bool status_word_for(cudaStream_t st, int **word) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  *word = g_status_ptrs[dev];
+  if (*word != nullptr) return true;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &capture) != cudaSuccess) return false;
+  if (capture != cudaStreamCaptureStatusNone) return true;
+  *word = status_word_ptr();
+  return *word != nullptr;
 }
 
 // Two words per vector-decay call.  [0]: raised by the one-reference vector-decay chunk kernels when a

@@ -81,5 +81,8 @@ struct CaptureRelaxed {
 // Address (on the current device) of the watchdog word that la_device_status() reads.
 // Defined in api.cu; kernels that can time out receive it as a parameter.
 int *status_word_ptr();
+// The same for kernels that do without the word where it cannot be had: looking it up for the first time on a device
+// would end a stream capture, so there the word stays null.  False on a CUDA error.
+bool status_word_for(cudaStream_t st, int **word);
 
 }  // namespace la

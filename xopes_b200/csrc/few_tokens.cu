@@ -260,7 +260,7 @@ int few_tokens_launch(const Product &p, int dtype, cudaStream_t st) {
     rc = make_map_2d(&g.w[i], p.b[i].p, dtype, p.K[0], p.N, p.b[i].ld, rows);
   if (rc != LA_OK) return rc;
   g.e = p.e;
-  g.status = status_word_ptr();
+  if (!status_word_for(st, &g.status)) return LA_ERR_CUDA;
   g.M = (int)p.M; g.N = (int)p.N;
   g.stages = (int)((p.K[0] + kStepK - 1) / kStepK);
   const int64_t tiles = (p.N + rows - 1) / rows;

@@ -439,7 +439,8 @@ int make_map_2d(CUtensorMap *m, const void *p, int dtype, int64_t inner, int64_t
   if (enc == nullptr) return LA_ERR_CUDA;
   static thread_local bool bound = false;  // the encoder needs the device's context current on this thread
   if (!bound) {
-    cudaFree(nullptr);
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return LA_ERR_CUDA;
     bound = true;
   }
   const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
@@ -530,7 +531,7 @@ int gemm_launch(const Product &p, const GemmPlan &plan, float *partial, int dtyp
   if (rc != LA_OK) return rc;
   g.e = p.e;
   g.partial = partial;
-  g.status = status_word_ptr();
+  if (!status_word_for(st, &g.status)) return LA_ERR_CUDA;
   g.M = (int)p.M; g.N = (int)p.N;
   const int cols = p.pair ? half : plan.bn;
   const int64_t mt = (p.M + kRows - 1) / kRows, nt = (p.N + cols - 1) / cols;

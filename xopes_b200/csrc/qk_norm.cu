@@ -706,8 +706,10 @@ int launch_stream(QkArgs &a, const bool (&mine)[2], cudaStream_t st) {
     a.items[k] = mine[k] ? a.T : 0;
   }
   share_ctas(a, (long long)sms * resident[dev]);
+  int *status = nullptr;
+  if (!status_word_for(st, &status)) return LA_ERR_CUDA;
   return launch_early(qk_norm_stream_kernel<T, BWD, INTER, VEC, LPR>, dim3(a.ctas[0] + a.ctas[1]), kThreads, kSmem, st, 0, a,
-                      status_word_ptr());
+                      status);
 }
 
 // Streamed: tensors whose heads lie next to each other and fill a warp's rows, from 2^20 elements on.  Measured, forward /

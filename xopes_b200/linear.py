@@ -75,6 +75,7 @@ class LinearFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        _lib.once_differentiable()
         lib = _lib.load()
         x, weight, z = ctx.saved_tensors
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
@@ -135,6 +136,7 @@ class GatedLinearFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dh):
+        _lib.once_differentiable()
         lib = _lib.load()
         x, w_gate, w_up, gu = ctx.saved_tensors
         need_x, need_wg, need_wu, need_bg, need_bu, _ = ctx.needs_input_grad
@@ -197,7 +199,8 @@ def linear_fn(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor
               residual: Optional[torch.Tensor] = None, act: str = "none") -> torch.Tensor:
     """y = act(x weight^T + bias) + residual, in one kernel.
 
-    x (..., K), weight (N, K), bias (N), residual (..., N), all of one dtype; rows may be strided (slices need no copy).
+    x (..., K), weight (N, K), bias (N), residual (..., N), all of one dtype; rows may be strided (slices need no copy; rows
+    of 16-bit tensors that do not start on 16 bytes, as with odd widths, are copied first).
     act: "none", "relu", "sigmoid", "silu" or "gelu" (the exact one, by erf).  The backward keeps x, the weight and,
     with an activation, the pre-activation (24 bits a value, fp32: 32)."""
     _check_bias(bias, weight.shape[0])

@@ -77,6 +77,7 @@ class QkNormRopeFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dqo, dko):
+        _lib.once_differentiable()
         lib = _lib.load()
         q, k, q_weight, k_weight, positions, cu = ctx.saved_tensors
         offset, freq, rotary_dim, interleaved, c, eps = ctx.cfg
@@ -118,7 +119,7 @@ def qk_norm_rope_fn(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.T
 
     q_weight, k_weight: (D,), shared by the heads; None = 1.
     positions: int64 (B,N), (1,N) or (N,); None counts from 0 in every sequence, or in every document of
-        cu_seqlens (M+1,) int64, batch 1.  offset is added (a host number; under a captured graph give positions).
+        cu_seqlens (M+1,) int64, batch 1 (tokens behind the last boundary count from it).  offset is added (a host number; under a captured graph give positions).
     rotary_dim: rotated features, the first of each head; even, D if None, 0 for the norm alone.
     inv_freq: rotary_dim / 2 host numbers, radians per position; base^(-2i / rotary_dim) if None.
     interleaved: pairs are features (2i, 2i+1) instead of (i, i + rotary_dim / 2).
