@@ -61,9 +61,14 @@ def _weights(q, q_weight, k_weight):
     dt = q.dtype
     if (q_weight is not None and q_weight.dtype != dt) or (k_weight is not None and k_weight.dtype != dt):
         dt = torch.float32
-    wq = None if q_weight is None else q_weight.to(dt).contiguous()
-    wk = None if k_weight is None else k_weight.to(dt).contiguous()
-    return wq, wk, _lib.LA_F32 if dt == torch.float32 else _lib.dtype_code(q)
+    return _as(q_weight, dt), _as(k_weight, dt), _lib.LA_F32 if dt == torch.float32 else _lib.dtype_code(q)
+
+
+def _as(t, dt):
+    """t contiguous and of type dt; the common case costs no call into torch's dispatcher."""
+    if t is None:
+        return None
+    return (t if t.dtype == dt else t.to(dt)).contiguous()
 
 
 class QkNormRopeFunction(torch.autograd.Function):
@@ -84,11 +89,10 @@ class QkNormRopeFunction(torch.autograd.Function):
         pos, pos_sb, pos_sn = _positions(positions)
         b, n, h, d = q.shape
         hk = k.shape[2]
-        dqo = torch.zeros(b, n, h, d, dtype=q.dtype, device=q.device) if dqo is None else dqo.to(q.dtype).contiguous()
-        dko = torch.zeros(b, n, hk, d, dtype=q.dtype, device=q.device) if dko is None else dko.to(q.dtype).contiguous()
+        dqo = torch.zeros((b, n, h, d), dtype=q.dtype, device=q.device) if dqo is None else _as(dqo, q.dtype)
+        dko = torch.zeros((b, n, hk, d), dtype=q.dtype, device=q.device) if dko is None else _as(dko, q.dtype)
         wq, wk, wcode = _weights(q, q_weight, k_weight)
-        dq = torch.empty(b, n, h, d, dtype=q.dtype, device=q.device)
-        dk = torch.empty(b, n, hk, d, dtype=q.dtype, device=q.device)
+        dq, dk = torch.empty_like(dqo), torch.empty_like(dko)
         dwq = torch.empty_like(wq) if wq is not None and ctx.needs_input_grad[2] else None
         dwk = torch.empty_like(wk) if wk is not None and ctx.needs_input_grad[3] else None
         ws, ws_bytes = None, 0
@@ -103,7 +107,7 @@ class QkNormRopeFunction(torch.autograd.Function):
                 _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dwq), _lib.ptr(dwk), _lib.ptr(ws), ws_bytes,
                 b, n, h, hk, d, rotary_dim, _lib.dtype_code(q), interleaved, c, eps, _lib.stream_of(q))
         _lib.check(rc, "la_qk_norm_rope_bwd")
-        return (dq, dk, None if dwq is None else dwq.to(q_weight.dtype), None if dwk is None else dwk.to(k_weight.dtype),
+        return (dq, dk, None if dwq is None else _as(dwq, q_weight.dtype), None if dwk is None else _as(dwk, k_weight.dtype),
                 None, None, None, None, None, None, None, None)
 
 
