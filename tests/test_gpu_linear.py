@@ -261,3 +261,25 @@ def test_two_streams_at_once():
             outs.append(gated_linear_fn(x, w, v))
     torch.cuda.synchronize()
     assert all(torch.equal(ref, o) for o in outs)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 results: the last rows of the output and of the gradients' operands."""
+    from xopes_b200.linear import linear_fn
+    m, k, n = 70000, 64, 32768
+    x = torch.zeros(m, k, device="cuda", dtype=torch.bfloat16)
+    x[-3:] = torch.randn(3, k, device="cuda")
+    w = (torch.randn(n, k, device="cuda") / 8).bfloat16()
+    leaf = x.clone().requires_grad_()
+    y = linear_fn(leaf, w, act="silu")
+    z = x[-3:].double() @ w.double().t()
+    close("y", F.silu(z), y[-3:], torch.bfloat16, x[-3:].double().abs() @ w.double().abs().t())
+    assert (y[:-3] == 0).all()
+    dy = torch.zeros(m, n, device="cuda", dtype=torch.bfloat16)
+    dy[-2:] = torch.randn(2, n, device="cuda")
+    dx, = torch.autograd.grad(y, leaf, dy)
+    dz = dy[-3:].double() * derivative(z, "silu")
+    e = HALF_STEP[torch.bfloat16] * (dz.abs() + 1.2 * (dy[-3:].double() * z).abs())
+    close("dx", dz @ w.double(), dx[-3:], torch.bfloat16, dz.abs() @ w.double().abs(),
+          float((e.square() @ w.double().square()).sum().sqrt()))
+    assert (dx[:-3] == 0).all()
