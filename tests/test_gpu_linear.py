@@ -115,6 +115,15 @@ def test_few_tokens(m, dtype):
     check(m, 1037, 75, dtype, train=False)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 4096, 4096), (8, 8192, 1000), (64, 4096, 1408), (128, 2048, 2048), (17, 11008, 512),
+                                   (100, 768, 9472), (40, 192, 20000)])
+def test_few_tokens_many_weights(m, k, n, dtype):
+    """Every size of a cluster and of its ring."""
+    check(m, k, n, dtype, "gelu", bias=True, residual=True, train=False)
+    check(m, k, n, dtype, "silu", pair=True, train=False)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("m,k,n", [(2048, 512, 768), (3000, 768, 2048), (515, 4096, 1024), (5000, 128, 128)])
 def test_larger(m, k, n, dtype):

@@ -7,8 +7,8 @@
 // a ring of TMA boxes, leaves its sums in its shared memory, and finishes a part of the tokens by adding up the sums of
 // all S through distributed shared memory, in order.  One launch, no scratch, equal calls give equal bits.
 //
-// Bound by HBM: 64 tokens through 2 x 11008 rows of 4096 (bf16) are 27.6 us at the measured copy bandwidth; 35.1 here, 49.7
-// with 256-token tiles and a second kernel for the splits of the contraction.  1 token, 4096 rows of 4096: 5.1, 10.5, 17.6.
+// Bound by HBM: 64 tokens through 2 x 11008 rows of 4096 (bf16) are 27.6 us at the measured copy bandwidth; 33.8 here, 49.7
+// with 256-token tiles and a second kernel for the splits of the contraction.  1 token, 4096 rows of 4096: 5.1, 9.2, 17.6.
 // What is left there is the launch, the first loads' way and the two cluster barriers; at 64 tokens the tokens' own boxes, which
 // every CTA reads from L2, take half of what the weights take.
 #include "linear.cuh"
@@ -24,14 +24,22 @@ using namespace la::ptx;
 constexpr int kRowsW = 128;               // weight rows of a CTA
 constexpr int kStepK = 64;
 constexpr int kMaxCluster = 8;
+constexpr int kMaxRing = 12;
+constexpr int kPerSm = 3;                 // CTAs of an SM, at most
 constexpr int kThreads = 192;             // warps: 0 loads, 1 multiplies, 2..5 read tensor memory and finish
 constexpr uint32_t kWBytes = kRowsW * 128;
 
 template <int MT> struct Cfg {            // MT: columns, the tokens rounded up to 16, 32, 64 or 128
   static constexpr uint32_t kStage = kWBytes + MT * 128;
-  static constexpr int kStages = MT <= 16 ? 4 : (MT <= 64 ? 3 : 2);   // three CTAs fit an SM
-  static constexpr uint32_t kRing = kStages * kStage;
-  static constexpr uint32_t kSmem = 1024 + kRing + 256;
+  static constexpr uint32_t kBeside = 1024 + 16 * kMaxRing + 64;  // alignment, barriers
+  // stages of a CTA's ring where `per_sm` of them share an SM's 228 KB (1 KB of each is the system's); the CTA's sums take
+  // its place in the end, MT x 512 bytes, which two stages hold
+  static int ring(int per_sm, int stages) {
+    int n = (int)((228u * 1024 / (unsigned)per_sm - 1024 - kBeside) / kStage);
+    if (n > stages) n = stages;
+    if (n > kMaxRing) n = kMaxRing;
+    return n < 2 ? 2 : n;
+  }
   static constexpr uint32_t kCols = MT < 32 ? 32 : MT;
 };
 
@@ -39,7 +47,7 @@ struct FewArgs {
   CUtensorMap w[2], x;
   Epilogue e;
   int *status;
-  int M, N, stages;
+  int M, N, stages, ring;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -80,7 +88,7 @@ __global__ void __launch_bounds__(kThreads) few_tokens_kernel(const __grid_const
   typedef Cfg<MT> C;
   extern __shared__ uint8_t raw[];
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
-  const uint32_t full = base + C::kRing, empty = full + 8 * C::kStages, done = empty + 8 * C::kStages;
+  const uint32_t full = base + g.ring * C::kStage, empty = full + 8 * g.ring, done = empty + 8 * g.ring;
   const uint32_t tmem_at = done + 8;
   volatile int *abort_flag = reinterpret_cast<volatile int *>(raw + (tmem_at + 4 - smem_u32(raw)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -90,7 +98,7 @@ __global__ void __launch_bounds__(kThreads) few_tokens_kernel(const __grid_const
 
   lets_next_start();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
+    for (int s = 0; s < g.ring; ++s) {
       mbar_init(full + 8 * s, 1);
       mbar_init(empty + 8 * s, 1);
     }
@@ -110,10 +118,9 @@ __global__ void __launch_bounds__(kThreads) few_tokens_kernel(const __grid_const
 
   bool ok = true;
   if (warp == 0) {
-    int it = 0;
-    for (int kb = k0; kb < k1 && ok; ++kb, ++it) {
-      const int s = it % C::kStages;
-      ok = warp_wait(empty + 8 * s, ((it / C::kStages) & 1) ^ 1, abort_flag, g.status, 321);
+    int s = 0, parity = 1;
+    for (int kb = k0; kb < k1; ++kb) {
+      ok = warp_wait(empty + 8 * s, parity, abort_flag, g.status, 321);
       if (!ok) break;
       const uint32_t ws = base + s * C::kStage, xs = ws + kWBytes, bar = full + 8 * s;
       const int k = kb * kStepK;
@@ -128,6 +135,10 @@ __global__ void __launch_bounds__(kThreads) few_tokens_kernel(const __grid_const
         load_box(xs, &g.x, bar, k, 0);
       }
       __syncwarp();
+      if (++s == g.ring) {
+        s = 0;
+        parity ^= 1;
+      }
     }
     if (!ok) {  // a wait gave up: let the copies in flight land
       const uint64_t t0 = globaltimer_ns();
@@ -135,20 +146,23 @@ __global__ void __launch_bounds__(kThreads) few_tokens_kernel(const __grid_const
     }
   } else if (warp == 1) {
     constexpr uint32_t idesc = instr_desc(tile::Fmt<T>::kAB, 0, 0, kRowsW, MT);
-    int it = 0;
-    for (int kb = k0; kb < k1 && ok; ++kb, ++it) {
-      const int s = it % C::kStages;
-      ok = warp_wait(full + 8 * s, (it / C::kStages) & 1, abort_flag, g.status, 322);
+    int s = 0, parity = 0;
+    for (int kb = k0; kb < k1; ++kb) {
+      ok = warp_wait(full + 8 * s, parity, abort_flag, g.status, 322);
       if (!ok) break;
       tc_fence_after();
       const uint32_t ws = base + s * C::kStage, xs = ws + kWBytes;
       if (elect_one()) {
 #pragma unroll
         for (int i = 0; i < kStepK / 16; ++i)
-          mma_ss(tmem, desc_kmajor(ws + i * 32), desc_kmajor(xs + i * 32), idesc, it > 0 || i > 0);
+          mma_ss(tmem, desc_kmajor(ws + i * 32), desc_kmajor(xs + i * 32), idesc, kb > k0 || i > 0);
         mma_commit(kb + 1 == k1 ? done : empty + 8 * s);
       }
       __syncwarp();
+      if (++s == g.ring) {
+        s = 0;
+        parity ^= 1;
+      }
     }
   } else {
     // the CTA's sums: [token][weight row], fp32, where the ring was (its last reader is done)
@@ -194,13 +208,15 @@ __global__ void __launch_bounds__(kThreads) few_tokens_kernel(const __grid_const
   if (warp == 1) tmem_dealloc(tmem, C::kCols);
 }
 
-// The cluster's size: the largest whose clusters all fit at once (more would leave a last round with few bytes in flight).
-// How many fit is asked for once per kernel and device; the answer counts one CTA an SM, three run there.  Measured with
-// sizes 1 .. 6 in us: 172 tiles of 4096 35 31.5 35 35 39 38 (2 taken), 148 tiles 32 28 33 32 31 35 (2), 96 tiles 27 21.2 20.8
-// 21.2 25 24 (4), 64 tiles of 8192 41 29 25.6 24.7 24.8 25.1 (6), 32 tiles of 4096 22 14.3 12.0 11.2 10.9 10.4 (8).  With more
-// stages and two CTAs an SM 172 tiles fitted with size 1 only, 34 us: some SMs had twice the work of others.
+// The cluster's size: the largest whose clusters all fit at once (more would leave a last round with few bytes in flight), of
+// at least three stages a CTA; from 64 tokens on 4 are enough for 32 tiles, since every token's sums come from all CTAs of a
+// cluster.  How many clusters fit is asked for once per kernel and device; the answer counts one CTA an SM, up to three
+// run there.  Measured with sizes 1 .. 8 in us, 1 token: 172 tiles of K 4096 32.5 31.3 34 34 37 37 40 39 (2 taken), 96 tiles 22.2
+// 20.4 19.3 19.4 23 23 24 23 (4), 64 tiles of K 8192 35 26 24.4 23.6 23.5 23.8 29 28 (6), 32 tiles of K 4096 19 12 10.3 10.3 9.7 9.6
+// 9.8 9.2 (8); 128 tokens, 32 tiles of K 4096: 32 21 17.7 14.5 16.3 16.0 17.9 17.7 (4), 16 tiles of K 2048: 23 16 13 10.3 10.6
+// 10.9 11.1 9.7 (8); 32 tokens, 32 tiles of K 768: 7.7 5.8 5.8 5.5 6.3 6.5 6.6 7.0 (4).
 template <typename T, int MT, bool PAIR>
-int launch_cfg(const FewArgs &g, int tiles, cudaStream_t st) {
+int launch_cfg(FewArgs g, int tiles, cudaStream_t st) {
   typedef Cfg<MT> C;
   static bool set[64] = {false};
   static int fit[64][kMaxCluster + 1];
@@ -208,7 +224,7 @@ int launch_cfg(const FewArgs &g, int tiles, cudaStream_t st) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return LA_ERR_CUDA;
   if (!set[dev]) {
     cudaError_t e = cudaFuncSetAttribute(few_tokens_kernel<T, MT, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)C::kSmem);
+                                         227 * 1024);
     for (int s = 1; s <= kMaxCluster && e == cudaSuccess; ++s) {
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -217,7 +233,7 @@ int launch_cfg(const FewArgs &g, int tiles, cudaStream_t st) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3((unsigned)s);
       cfg.blockDim = dim3(kThreads);
-      cfg.dynamicSmemBytes = C::kSmem;
+      cfg.dynamicSmemBytes = C::kBeside + C::ring(kPerSm, kMaxRing) * C::kStage;
       cfg.attrs = attr;
       cfg.numAttrs = 1;
       e = cudaOccupancyMaxActiveClusters(&fit[dev][s], few_tokens_kernel<T, MT, PAIR>, &cfg);
@@ -229,9 +245,15 @@ int launch_cfg(const FewArgs &g, int tiles, cudaStream_t st) {
     }
     set[dev] = true;
   }
-  int size = g.stages < kMaxCluster ? g.stages : kMaxCluster;
-  while (size > 1 && 3 * fit[dev][size] < tiles) --size;
-  return launch_early(few_tokens_kernel<T, MT, PAIR>, dim3((unsigned)(tiles * size)), kThreads, C::kSmem, st, size, g);
+  int size = MT >= 64 && tiles >= 32 ? 4 : kMaxCluster;
+  if (size > g.stages / 3) size = g.stages < 3 ? 1 : g.stages / 3;
+  while (size > 1 && kPerSm * fit[dev][size] < tiles) --size;
+  // few CTAs an SM: the more stages each
+  int per_sm = (tiles + fit[dev][size] - 1) / fit[dev][size];
+  if (per_sm > kPerSm) per_sm = kPerSm;
+  g.ring = C::ring(per_sm, (g.stages + size - 1) / size);
+  return launch_early(few_tokens_kernel<T, MT, PAIR>, dim3((unsigned)(tiles * size)), kThreads,
+                      C::kBeside + g.ring * C::kStage, st, size, g);
 }
 
 template <typename T, bool PAIR>
