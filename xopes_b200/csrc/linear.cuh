@@ -164,18 +164,20 @@ struct Epilogue {
   int vec;  // every pointer 16-byte aligned, every row stride and save_up a multiple of 16 bytes in the type of x
 };
 
-// W consecutive elements (W sizeof(T) = 8 or a multiple of 16 bytes) from / to p; `left` of them exist
+// W consecutive elements from / to p, `left` of them exist; vec: in accesses of 8 or 16 bytes where W elements fill them
 template <typename T, int W>
 __device__ __forceinline__ void load_row(const T *p, bool vec, int left, float (&v)[W]) {
-  if (vec && left >= W) {
-    constexpr int kBytes = W * (int)sizeof(T);
-    if constexpr (kBytes == 8) {
+  constexpr int kBytes = W * (int)sizeof(T), kPer = 16 / (int)sizeof(T);
+  if constexpr (kBytes == 8) {
+    if (vec && left >= W) {
       const uint2 r = *reinterpret_cast<const uint2 *>(p);
       const T *h = reinterpret_cast<const T *>(&r);
 #pragma unroll
       for (int j = 0; j < W; ++j) v[j] = Cvt<T>::to_f(h[j]);
-    } else {
-      constexpr int kPer = 16 / (int)sizeof(T);
+      return;
+    }
+  } else if constexpr (kBytes % 16 == 0) {
+    if (vec && left >= W) {
 #pragma unroll
       for (int i = 0; i < W / kPer; ++i) {
         const uint4 r = *reinterpret_cast<const uint4 *>(p + i * kPer);
@@ -183,24 +185,26 @@ __device__ __forceinline__ void load_row(const T *p, bool vec, int left, float (
 #pragma unroll
         for (int j = 0; j < kPer; ++j) v[i * kPer + j] = Cvt<T>::to_f(h[j]);
       }
+      return;
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < W; ++j) v[j] = j < left ? Cvt<T>::to_f(p[j]) : 0.f;
   }
+#pragma unroll
+  for (int j = 0; j < W; ++j) v[j] = j < left ? Cvt<T>::to_f(p[j]) : 0.f;
 }
 template <typename T, int W>
 __device__ __forceinline__ void store_row(T *p, bool vec, int left, const float (&v)[W]) {
-  if (vec && left >= W) {
-    constexpr int kBytes = W * (int)sizeof(T);
-    if constexpr (kBytes == 8) {
+  constexpr int kBytes = W * (int)sizeof(T), kPer = 16 / (int)sizeof(T);
+  if constexpr (kBytes == 8) {
+    if (vec && left >= W) {
       uint2 r;
       T *h = reinterpret_cast<T *>(&r);
 #pragma unroll
       for (int j = 0; j < W; ++j) h[j] = Cvt<T>::from_f(v[j]);
       *reinterpret_cast<uint2 *>(p) = r;
-    } else {
-      constexpr int kPer = 16 / (int)sizeof(T);
+      return;
+    }
+  } else if constexpr (kBytes % 16 == 0) {
+    if (vec && left >= W) {
 #pragma unroll
       for (int i = 0; i < W / kPer; ++i) {
         uint4 r;
@@ -209,12 +213,12 @@ __device__ __forceinline__ void store_row(T *p, bool vec, int left, const float 
         for (int j = 0; j < kPer; ++j) h[j] = Cvt<T>::from_f(v[i * kPer + j]);
         *reinterpret_cast<uint4 *>(p + i * kPer) = r;
       }
+      return;
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < W; ++j)
-      if (j < left) p[j] = Cvt<T>::from_f(v[j]);
   }
+#pragma unroll
+  for (int j = 0; j < W; ++j)
+    if (j < left) p[j] = Cvt<T>::from_f(v[j]);
 }
 
 // W kept values at offset `off` (W a multiple of 8 where vec is set for a 16-bit type)
