@@ -14,8 +14,9 @@
 //
 // Warps: 0 loads, 1 multiplies (one elected lane of the first CTA for both), 2 owns tensor memory, 4..11 write.  Two
 // accumulators: while one tile is written the next is multiplied.  Persistent: one pair of CTAs per two SMs, tiles in
-// groups of 8 rows of tiles, so that the operands of the tiles in flight stay in L2.  Where there are fewer tiles than
-// SMs the contraction is split over several units, whose fp32 sums another kernel adds in a fixed order (gemm_plan).
+// groups of 8 rows of tiles, so that the operands of the tiles in flight stay in L2.  Tiles that do not fill a round of the
+// pairs (all of them where there are few, else the last round's) have their contraction split over several units, whose
+// fp32 sums tile_sum_kernel adds in a fixed order (gemm_plan).
 //
 // Every wait is bounded (mbar_wait); one that runs out ends the kernel with the device's status word set.
 #include "linear.cuh"
@@ -48,11 +49,13 @@ template <int BN> struct Cfg {
 struct GemmArgs {
   CUtensorMap a[2], b[2];
   Epilogue e;
-  float *partial;
+  float *partial;            // sums of split tiles: [tile - whole][split][row][BN]
   int *status;
   int M, N;
   int kb[2];                 // stages of each segment
-  int m_tiles, n_tiles, splits;
+  int m_tiles, n_tiles;
+  int whole, splits;         // tiles [0, whole) are done whole, the others in `splits` units each
+  int rows;                  // rows of a split tile
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -99,20 +102,26 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 }
 
 struct Unit {
-  int m0, n0, k0, k1, split;
+  int m0, n0, k0, k1;
+  int slot;  // place of its sums, or -1 for a whole tile
 };
-template <int BN, bool PAIR>
-__device__ __forceinline__ Unit unit_of(const GemmArgs &g, int u) {
-  const int tile = u / g.splits, split = u - tile * g.splits;
+template <int BN, bool PAIR> __device__ __forceinline__ void place_of(const GemmArgs &g, int tile, int &m0, int &n0) {
   const int per = kGroup * g.n_tiles, group = tile / per, first = group * kGroup;
   const int rows = min(g.m_tiles - first, kGroup), r = tile - group * per;
+  m0 = (first + r % rows) * kRows;
+  n0 = r / rows * (PAIR ? BN / 2 : BN);
+}
+template <int BN, bool PAIR>
+__device__ __forceinline__ Unit unit_of(const GemmArgs &g, int u) {
+  const int v = u - g.whole;
+  const bool cut = v >= 0;
+  const int part = cut ? v / g.splits : 0, split = v - part * g.splits;
   Unit x;
-  x.m0 = (first + r % rows) * kRows;
-  x.n0 = r / rows * (PAIR ? BN / 2 : BN);
-  const long long all = g.kb[0] + g.kb[1];
-  x.k0 = (int)(all * split / g.splits);
-  x.k1 = (int)(all * (split + 1) / g.splits);
-  x.split = split;
+  place_of<BN, PAIR>(g, cut ? g.whole + part : u, x.m0, x.n0);
+  const int all = g.kb[0] + g.kb[1];
+  x.k0 = cut ? (int)((long long)all * split / g.splits) : 0;
+  x.k1 = cut ? (int)((long long)all * (split + 1) / g.splits) : all;
+  x.slot = cut ? v : -1;
   return x;
 }
 
@@ -232,23 +241,22 @@ __device__ __noinline__ void edge_strip(const Epilogue &e, float *strip, long lo
   }
 }
 
-// a strip of one split's sums
-template <bool PAIR>
-__device__ __noinline__ void partial_strip(const GemmArgs &g, float *strip, int split, long long m0, int n0, int lane) {
+// a strip of a split tile's sums: rows r0 .. r0 + 31 of the tile, accumulator columns from c (and for u from c2) on
+template <bool PAIR, int BN>
+__device__ __noinline__ void sums_strip(const GemmArgs &g, float *strip, int slot, int r0, int c, int c2, int lane) {
   typedef Strip<PAIR> S;
-  const int cl = lane % S::kLanes, rl = lane / S::kLanes, col = n0 + 8 * cl, left = g.N - col;
-  const bool vec = g.N % 4 == 0;
-  float *o = g.partial + ((long long)split * (PAIR ? 2 : 1) * g.M + m0 + rl) * g.N + col;
+  const int cl = lane % S::kLanes, rl = lane / S::kLanes;
+  float *o = g.partial + ((long long)slot * g.rows + r0 + rl) * BN + 8 * cl;
 #pragma unroll 4
-  for (int i = 0; i < S::kLanes; ++i, o += (long long)S::kRowsAt * g.N) {
+  for (int i = 0; i < S::kLanes; ++i, o += S::kRowsAt * BN) {
     const int row = i * S::kRowsAt + rl;
-    if (m0 + row >= g.M || left <= 0) break;
+    if (r0 + row >= g.rows) break;
     float p[8];
     S::take(strip, row, cl, 0, p);
-    store_row<float, 8>(o, vec, left, p);
+    store_row<float, 8>(o + c, true, 8, p);
     if (PAIR) {
       S::take(strip, row, cl, 1, p);
-      store_row<float, 8>(o + (long long)g.M * g.N, vec, left, p);
+      store_row<float, 8>(o + c2, true, 8, p);
     }
   }
 }
@@ -265,7 +273,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   volatile int *abort_flag = reinterpret_cast<volatile int *>(raw + (tmem_at + 4 - smem_u32(raw)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
-  const int units = g.m_tiles * g.n_tiles * g.splits;
+  const int units = g.whole + (g.m_tiles * g.n_tiles - g.whole) * g.splits;
   const int first = blockIdx.x >> 1, stride = gridDim.x >> 1;
 
   lets_next_start();
@@ -410,8 +418,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         }
         __syncwarp();
         const bool inner = n0 + Strip<PAIR>::kCols <= g.N && m0 + 32 <= g.M;
-        if (g.partial != nullptr) {
-          partial_strip<PAIR>(g, strip, x.split, m0, n0, lane);
+        if (x.slot >= 0) {
+          sums_strip<PAIR, BN>(g, strip, x.slot, (int)rank * 128 + quarter * 32, c, c + kOut, lane);
         } else {
           T *out = inner && g.e.vec ? out_rows<T>(g.e, m0) : nullptr;
           if (out != nullptr) inner_strip<T, PAIR>(g.e, strip, out, m0, n0, lane);
@@ -430,6 +438,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
   tc_fence_after();
   if (warp == 2)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kCols) : "memory");
+}
+
+// The sums of a split tile's units, in order, and the epilogue.  CTA (split tile, 8 rows), 8 columns a thread.
+template <typename T, int BN, bool PAIR>
+__global__ void __launch_bounds__(256) tile_sum_kernel(const __grid_constant__ GemmArgs g) {
+  constexpr int kLanes = (PAIR ? BN / 2 : BN) / 8;
+  lets_next_start();
+  after_previous();
+  int m0, n0;
+  place_of<BN, PAIR>(g, g.whole + (int)blockIdx.x, m0, n0);
+  for (int j = threadIdx.x; j < 8 * kLanes; j += 256) {
+    const int row = (int)blockIdx.y * 8 + j / kLanes, col = j % kLanes * 8;
+    if (row >= g.rows || m0 + row >= g.M || n0 + col >= g.N) continue;
+    const float *s = g.partial + ((long long)blockIdx.x * g.splits * g.rows + row) * BN + col;
+    float p[8] = {}, q[8] = {};
+    const long long step = (long long)g.rows * BN;
+    for (int i = 0; i < g.splits; i += 4) {  // four units' loads at a time, added in order
+      float v[4][8], w[4][8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool is = i + j < g.splits;
+        load_row<float, 8>(s + (is ? j * step : 0), true, 8, v[j]);
+        if (PAIR) load_row<float, 8>(s + (is ? j * step : 0) + BN / 2, true, 8, w[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (i + j >= g.splits) break;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          p[k] += v[j][k];
+          if (PAIR) q[k] += w[j][k];
+        }
+      }
+      s += 4 * step;
+    }
+    if (PAIR) finish_pair<T, 8>(g.e, m0 + row, n0 + col, g.N, p, q);
+    else finish_one<T, 8>(g.e, m0 + row, n0 + col, g.N, p);
+  }
 }
 
 }  // namespace
@@ -480,7 +526,10 @@ int launch_cfg(const GemmArgs &g, int units, cudaStream_t st) {
   }
   const int pairs = sm_count() / 2;
   const int grid = 2 * (units < pairs ? units : pairs);
-  return launch_early(gemm_kernel<T, A_MN, B_MN, BN, PAIR>, dim3((unsigned)grid), kThreads, C::kSmem, st, 0, g);
+  const int rc = launch_early(gemm_kernel<T, A_MN, B_MN, BN, PAIR>, dim3((unsigned)grid), kThreads, C::kSmem, st, 0, g);
+  const int cut = g.m_tiles * g.n_tiles - g.whole;
+  if (rc != LA_OK || cut == 0) return rc;
+  return launch_early(tile_sum_kernel<T, BN, PAIR>, dim3((unsigned)cut, (unsigned)((g.rows + 7) / 8)), 256, 0, st, 0, g);
 }
 
 template <typename T, int BN>
@@ -495,25 +544,35 @@ int launch_t(const Product &p, const GemmArgs &g, int units, cudaStream_t st) {
 
 }  // namespace
 
+// Estimates the kernel's time for tiles of 256 and 128 columns, whole or split: every tile in s units, or the tiles of the last,
+// incomplete round in as many units as there are pairs for.  A stage takes 0.28 us (256 columns) or 0.20, a tile 0.5 us
+// besides, sums another launch (2.5 us) and their way to memory and back (4 TB/s).  Against measurements of 17 shapes with
+// 1 .. 16 units a tile the estimate's choice was the quickest or within 4 % of it in 15, within 9 % in all.
 GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K0, int64_t K1, bool pair) {
   const int64_t pairs = sm_count() / 2;
-  const int64_t mt = (M + kRows - 1) / kRows;
+  const int64_t mt = (M + kRows - 1) / kRows, rows = M < kRows ? M : kRows;
   const int64_t kb = (K0 + kStepK - 1) / kStepK + (K1 + kStepK - 1) / kStepK;
-  GemmPlan best = {256, 1};
+  GemmPlan best = {};
   double best_us = 1e30;
   for (int bn = 256; bn >= 128; bn /= 2) {
     const int64_t cols = pair ? bn / 2 : bn;
     const int64_t tiles = mt * ((N + cols - 1) / cols);
-    const double step = bn == 256 ? 0.28 : 0.20;  // us a stage
-    for (int64_t s = 1; s <= 16 && s * 4 <= kb + 3; ++s) {
-      if (s > 1 && tiles * (s - 1) >= pairs * 4) break;
-      const int64_t waves = (tiles * s + pairs - 1) / pairs;
-      double us = waves * ((kb + s - 1) / s * step + 0.5) + 2.0;
-      if (s > 1) us += 2.5 + (double)s * M * N * (pair ? 2 : 1) * 8 / 4e6;
-      if (us < best_us) {
-        best_us = us;
-        best = GemmPlan{bn, (int)s};
+    const double step = bn == 256 ? 0.28 : 0.20;
+    auto consider = [&](int64_t whole, int64_t s) {
+      const int64_t cut = (tiles - whole) * s;
+      double us = 2.0 + (whole + pairs - 1) / pairs * (kb * step + 0.5);
+      if (cut > 0) {
+        const double most = (double)s * M * N * (pair ? 2 : 1), sums = (double)cut * rows * bn;  // rows past M are not written
+        us += (cut + pairs - 1) / pairs * ((kb + s - 1) / s * step + 0.5) + 2.5 + (sums < most ? sums : most) * 8 / 4e6;
       }
+      if (us >= best_us) return;
+      best_us = us;
+      best = GemmPlan{bn, (int)s, whole, rows, cut * rows * bn * 4};
+    };
+    consider(tiles, 1);
+    for (int64_t s = 2; s <= 16 && s * 4 <= kb + 3; ++s) {
+      if (tiles * (s - 1) < pairs * 4) consider(0, s);
+      if (tiles > pairs && tiles % pairs * s <= pairs) consider(tiles / pairs * pairs, s);
     }
   }
   return best;
@@ -535,9 +594,11 @@ int gemm_launch(const Product &p, const GemmPlan &plan, float *partial, int dtyp
   g.M = (int)p.M; g.N = (int)p.N;
   const int cols = p.pair ? half : plan.bn;
   const int64_t mt = (p.M + kRows - 1) / kRows, nt = (p.N + cols - 1) / cols;
-  if (mt * nt * plan.splits > INT32_MAX / 2) return LA_ERR_TOO_LARGE;
-  g.m_tiles = (int)mt; g.n_tiles = (int)nt; g.splits = plan.splits;
-  const int units = (int)(mt * nt * plan.splits);
+  const int64_t all = plan.whole + (mt * nt - plan.whole) * plan.splits;
+  if (all > INT32_MAX / 2) return LA_ERR_TOO_LARGE;
+  g.m_tiles = (int)mt; g.n_tiles = (int)nt;
+  g.whole = (int)plan.whole; g.splits = plan.splits; g.rows = (int)plan.rows;
+  const int units = (int)all;
   if (dtype == LA_BF16)
     return plan.bn == 256 ? launch_t<__nv_bfloat16, 256>(p, g, units, st) : launch_t<__nv_bfloat16, 128>(p, g, units, st);
   return plan.bn == 256 ? launch_t<__half, 256>(p, g, units, st) : launch_t<__half, 128>(p, g, units, st);

@@ -277,9 +277,9 @@ __global__ void __launch_bounds__(256) few_tokens_fp32_kernel(const float *x, lo
   else finish_one<float, 1>(e, m, (int)n, N, p);
 }
 
-// ------------------------------------------------------------------------------ sums over the splits
+// ------------------------------------------------------------------------------ sums over the splits of an fp32 product
 // out of the partial products (splits, PAIR ? 2 : 1, M, N) in a fixed order, then the epilogue; 8 columns a thread
-template <typename T, bool PAIR>
+template <bool PAIR>
 __global__ void __launch_bounds__(256) split_sum_kernel(const float *partial, int splits, long long M, int N, Epilogue e) {
   constexpr int W = 8;
   lets_next_start();
@@ -306,8 +306,8 @@ __global__ void __launch_bounds__(256) split_sum_kernel(const float *partial, in
       p += mat;
     }
   }
-  if (PAIR) finish_pair<T, W>(e, m, n, N, g, u);
-  else finish_one<T, W>(e, m, n, N, g);
+  if (PAIR) finish_pair<float, W>(e, m, n, N, g, u);
+  else finish_one<float, W>(e, m, n, N, g);
 }
 
 // ------------------------------------------------------------------------------ derivative of the activation
@@ -588,11 +588,10 @@ int few_fp32_launch(const Product &p, cudaStream_t st) {
                       p.a[0].ld, w0, p.b[0].ld, w1, p.b[1].ld, (int)p.M, (int)p.N, (int)p.K[0], share, e);
 }
 
-template <typename T>
 int split_sum_launch(const Product &p, int splits, const float *partial, cudaStream_t st) {
   const int64_t grid = (p.M * ((p.N + 7) / 8) + 255) / 256;
   if (grid > INT32_MAX) return LA_ERR_TOO_LARGE;
-  return launch_early(p.pair ? split_sum_kernel<T, true> : split_sum_kernel<T, false>, dim3((unsigned)grid), 256, 0, st, 0, partial,
+  return launch_early(p.pair ? split_sum_kernel<true> : split_sum_kernel<false>, dim3((unsigned)grid), 256, 0, st, 0, partial,
                       splits, p.M, (int)p.N, p.e);
 }
 
@@ -626,27 +625,23 @@ int product(Product p, int dtype, Scratch s, int64_t &need, cudaStream_t st) {
     if (p.M == 2) return few_fp32_launch<2>(p, st);
     return p.M <= 4 ? few_fp32_launch<4>(p, st) : few_fp32_launch<8>(p, st);
   }
-  GemmPlan plan = {0, 1};
-  SimtPlan simt = {0, 1};
+  GemmPlan plan = {};
+  SimtPlan simt = {};
+  int64_t bytes = 0;
   if (dtype == LA_F32) {
     simt = simt_plan(p);
-    plan.splits = simt.splits;
+    if (simt.splits > 1) bytes = (int64_t)simt.splits * (p.pair ? 2 : 1) * p.M * p.N * 4;
   } else {
     plan = gemm_plan(p.M, p.N, p.K[0], p.segments > 1 ? p.K[1] : 0, p.pair != 0);
+    bytes = plan.partial_bytes;
   }
-  float *partial = nullptr;
-  if (plan.splits > 1) partial = static_cast<float *>(s.take((int64_t)plan.splits * (p.pair ? 2 : 1) * p.M * p.N * 4));
+  float *partial = bytes > 0 ? static_cast<float *>(s.take(bytes)) : nullptr;
   if (s.used > need) need = s.used;
   if (s.base == nullptr) return LA_OK;
   p.e.vec = epilogue_vec(p.e, dtype);
-  const int rc = dtype == LA_F32 ? simt_launch(p, simt, partial, st) : gemm_launch(p, plan, partial, dtype, st);
-  if (rc != LA_OK || partial == nullptr) return rc;
-  switch (dtype) {
-    case LA_F32: return split_sum_launch<float>(p, plan.splits, partial, st);
-    case LA_BF16: return split_sum_launch<__nv_bfloat16>(p, plan.splits, partial, st);
-    case LA_F16: return split_sum_launch<__half>(p, plan.splits, partial, st);
-  }
-  return LA_ERR_UNSUPPORTED;
+  if (dtype != LA_F32) return gemm_launch(p, plan, partial, dtype, st);
+  const int rc = simt_launch(p, simt, partial, st);
+  return rc != LA_OK || partial == nullptr ? rc : split_sum_launch(p, simt.splits, partial, st);
 }
 
 template <typename T, int VEC>

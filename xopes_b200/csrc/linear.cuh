@@ -349,10 +349,11 @@ struct Product {
 
 int sm_count();  // of the current device (148 where there is none); linear.cu
 
-// gemm_sm100.cu.  Number of splits of the contraction (partial sums in fp32, finished by another launch), its
-// workspace, and the launch.  16-bit operands with 16-byte aligned addresses and row strides.
+// gemm_sm100.cu, for 16-bit operands with 16-byte aligned addresses and row strides: columns of a tile, units of a split tile,
+// tiles that are done whole, rows of a split tile, and the workspace for their sums.
 struct GemmPlan {
   int bn, splits;
+  int64_t whole, rows, partial_bytes;
 };
 GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K0, int64_t K1, bool pair);
 int gemm_launch(const Product &p, const GemmPlan &plan, float *partial, int dtype, cudaStream_t st);
