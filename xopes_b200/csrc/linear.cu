@@ -1,5 +1,5 @@
 // linear_fn and gated_linear_fn: the host plan of both directions, the fp32 product, and the passes around the
-// matrix products (derivative of the activation, sums over rows, sums over the splits of a contraction).
+// matrix products (derivative of the activation, sums over rows).
 //
 //   linear        z = x W^T + b             y = act(z) + r
 //                 dz = dy act'(z)           dx = dz W      dW = dz^T x      db = sum over rows of dz
@@ -45,9 +45,20 @@ struct SimtArgs {
   long long M, N;
   int n_tiles, splits;
   long long steps[2];  // 16-wide steps of each segment
-  float *partial;      // (splits, pair ? 2 : 1, M, N) or null
   Epilogue e;
 };
+
+__device__ __forceinline__ void cluster_all() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// four floats at this CTA's shared address `at`, of the cluster's CTA `rank`
+__device__ __forceinline__ float4 load_of(uint32_t at, uint32_t rank) {
+  float4 v;
+  asm volatile(
+      "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [r];\n\t}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at), "r"(rank) : "memory");
+  return v;
+}
 
 constexpr int kStep = 16;
 template <int TILE> constexpr int simt_threads() { return TILE == 128 ? 256 : 128; }
@@ -107,13 +118,25 @@ __device__ __forceinline__ void simt_put(bool mn, float (*s)[TILE + 4], const fl
 }
 
 // One TILE x TILE tile (of one split) per CTA, 8 x 4 results a thread (TILE 64, 128 threads) or 8 x 8 (TILE 128, 256 threads),
-// packed over pairs of rows; the next step's operands are in registers while the current step's are multiplied.
-// 2048 x 2048 x 2048 426 us (40 TFLOP/s; the instructions beside the products and shared memory bound it; elements of B kept
-// twice in shared memory, to save doubling them in registers, 860 us), 514 x 512 x 512 17.5 us with the sum of the splits.
+// packed over pairs of rows; the next step's operands are in registers while the current step's are multiplied.  The splits
+// of a tile are a cluster: each CTA adds everyone's sums for a part of the tile, in order, out of shared memory.  2048 x 2048 x
+// 2048 416 us (41 TFLOP/s; the instructions beside the products and shared memory bound it; elements of B kept twice in shared
+// memory, to save doubling them in registers, 860 us).  514 x 512 x 512 14.6 us, 128 x 16384 x 128 57; with the splits' sums
+// through global memory and a second launch 16.7 and 61, but 16 x 4096 x 4096 61 instead of 70 (clusters of 9 fill the SMs
+// less evenly).
 template <int TILE, bool PAIR>
 __global__ void __launch_bounds__(simt_threads<TILE>(), TILE == 128 ? 2 : (PAIR ? 3 : 5)) simt_product_kernel(const SimtArgs a) {
   constexpr int TN = TILE / 16;  // columns a thread: 4 from tx * 4 on, and for TILE 128 4 from 64 + tx * 4 on
-  __shared__ __align__(16) float sa[2][kStep][TILE + 4], sb[2][PAIR ? 2 : 1][kStep][TILE + 4];
+  constexpr int P = PAIR ? 2 : 1;
+  union Shared {
+    struct {
+      float a[2][kStep][TILE + 4], b[2][P][kStep][TILE + 4];
+    } in;
+    float4 sums[P][TILE][16];  // 64 columns
+  };
+  __shared__ __align__(16) Shared mem;
+  auto &sa = mem.in.a;
+  auto &sb = mem.in.b;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const long long tile = blockIdx.x / a.splits;
   const int split = (int)(blockIdx.x - tile * a.splits);
@@ -180,30 +203,57 @@ __global__ void __launch_bounds__(simt_threads<TILE>(), TILE == 128 ? 2 : (PAIR 
     if (s + 1 < s1) put(at ^ 1);
     __syncthreads();
   }
+  auto take = [&](int i, int h, float (&p)[4], float (&q)[4]) {  // row i, columns 4 h .. 4 h + 3 of this thread
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+    for (int j = 0; j < 4; ++j) {
+      p[j] = i % 2 ? acc[i / 2][4 * h + j].y : acc[i / 2][4 * h + j].x;
+      q[j] = i % 2 ? acc2[PAIR ? i / 2 : 0][4 * h + j].y : acc2[PAIR ? i / 2 : 0][4 * h + j].x;
+    }
+  };
+  auto finish = [&](long long m, long long n, float (&p)[4], float (&q)[4]) {
+    if (m >= a.M || n >= a.N) return;
+    if (PAIR) finish_pair<float, 4>(a.e, m, (int)n, (int)a.N, p, q);
+    else finish_one<float, 4>(a.e, m, (int)n, (int)a.N, p);
+  };
+  if (a.splits == 1) {
 #pragma unroll
-    for (int h = 0; h < TN / 4; ++h) {
-      const long long m = m0 + ty * 8 + i, n = n0 + tx * 4 + 64 * h;
-      if (m >= a.M || n >= a.N) continue;
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int h = 0; h < TN / 4; ++h) {
+        float p[4], q[4];
+        take(i, h, p, q);
+        finish(m0 + ty * 8 + i, n0 + tx * 4 + 64 * h, p, q);
+      }
+    return;
+  }
+#pragma unroll
+  for (int h = 0; h < TN / 4; ++h) {
+    if (h > 0) cluster_all();  // the first 64 columns have been read
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
       float p[4], q[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        p[j] = i % 2 ? acc[i / 2][4 * h + j].y : acc[i / 2][4 * h + j].x;
-        q[j] = i % 2 ? acc2[PAIR ? i / 2 : 0][4 * h + j].y : acc2[PAIR ? i / 2 : 0][4 * h + j].x;
+      take(i, h, p, q);
+      mem.sums[0][ty * 8 + i][tx] = make_float4(p[0], p[1], p[2], p[3]);
+      if (PAIR) mem.sums[P - 1][ty * 8 + i][tx] = make_float4(q[0], q[1], q[2], q[3]);
+    }
+    cluster_all();
+    for (int u = split * simt_threads<TILE>() + threadIdx.x; u < TILE * 16; u += a.splits * simt_threads<TILE>()) {
+      if (m0 + (u >> 4) >= a.M) break;
+      const uint32_t at = (uint32_t)__cvta_generic_to_shared(&mem.sums[0][u >> 4][u & 15]);
+      float p[4] = {}, q[4] = {};
+#pragma unroll 4
+      for (int i = 0; i < a.splits; ++i) {
+        const float4 v = load_of(at, i);
+        p[0] += v.x; p[1] += v.y; p[2] += v.z; p[3] += v.w;
+        if (PAIR) {
+          const float4 w = load_of(at + TILE * 256u, i);
+          q[0] += w.x; q[1] += w.y; q[2] += w.z; q[3] += w.w;
+        }
       }
-      if (a.partial != nullptr) {
-        float *o = a.partial + ((long long)split * (PAIR ? 2 : 1) * a.M + m) * a.N + n;
-        const int left = (int)(a.N - n < 4 ? a.N - n : 4);
-        store_row<float, 4>(o, a.N % 4 == 0, left, p);
-        if (PAIR) store_row<float, 4>(o + a.M * a.N, a.N % 4 == 0, left, q);
-      } else if (PAIR) {
-        finish_pair<float, 4>(a.e, m, (int)n, (int)a.N, p, q);
-      } else {
-        finish_one<float, 4>(a.e, m, (int)n, (int)a.N, p);
-      }
+      finish(m0 + (u >> 4), n0 + (u & 15) * 4 + 64 * h, p, q);
     }
   }
+  cluster_all();  // the sums stay until everyone has read them
 }
 
 // Up to 8 tokens in fp32: the weights' bytes are the work.  A warp streams four weight rows (two of each of a pair) and keeps
@@ -275,39 +325,6 @@ __global__ void __launch_bounds__(256) few_tokens_fp32_kernel(const float *x, lo
   if (m >= M || n >= N) return;
   if (PAIR) finish_pair<float, 1>(e, m, (int)n, N, p, q);
   else finish_one<float, 1>(e, m, (int)n, N, p);
-}
-
-// ------------------------------------------------------------------------------ sums over the splits of an fp32 product
-// out of the partial products (splits, PAIR ? 2 : 1, M, N) in a fixed order, then the epilogue; 8 columns a thread
-template <bool PAIR>
-__global__ void __launch_bounds__(256) split_sum_kernel(const float *partial, int splits, long long M, int N, Epilogue e) {
-  constexpr int W = 8;
-  lets_next_start();
-  after_previous();
-  const int packs = (N + W - 1) / W;
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= M * packs) return;
-  const long long m = i / packs;
-  const int n = (int)(i - m * packs) * W, left = N - n;
-  const bool vec = N % 4 == 0;
-  const long long mat = M * N;
-  float g[W] = {}, u[W] = {};
-  const float *p = partial + m * N + n;
-  for (int s = 0; s < splits; ++s) {
-    float v[W];
-    load_row<float, W>(p, vec, left, v);
-#pragma unroll
-    for (int j = 0; j < W; ++j) g[j] += v[j];
-    p += mat;
-    if (PAIR) {
-      load_row<float, W>(p, vec, left, v);
-#pragma unroll
-      for (int j = 0; j < W; ++j) u[j] += v[j];
-      p += mat;
-    }
-  }
-  if (PAIR) finish_pair<float, W>(e, m, n, N, g, u);
-  else finish_one<float, W>(e, m, n, N, g);
 }
 
 // ------------------------------------------------------------------------------ derivative of the activation
@@ -525,7 +542,7 @@ int epilogue_vec(const Epilogue &e, int dtype) {
 
 // Tile and splits of an fp32 product.  Tiles of 128 where the result is wider than 64 both ways and they and their splits
 // fill the GPU, else of 64; splits for two (tiles of 128) or four CTAs an SM, of at least 256 or 64 terms.  With tiles of 64 /
-// of 128: 1024 x 1024 x 1024 73 / 63 us, 700 x 2000 x 3008 250 / 207, 16 x 4096 x 4096 65 / 101.
+// of 128: 1024 x 1024 x 1024 79 / 59 us, 700 x 2000 x 3000 286 / 202, 16 x 4096 x 4096 70 / 141.
 struct SimtPlan {
   int tile, splits;
 };
@@ -547,7 +564,27 @@ SimtPlan simt_plan(const Product &p) {
   return plan(64, 4, 64);
 }
 
-int simt_launch(const Product &p, const SimtPlan &plan, float *partial, cudaStream_t st) {
+template <int TILE, bool PAIR>
+int simt_launch_tile(const SimtArgs &a, int64_t grid, cudaStream_t st) {
+  if (a.splits > 8) {  // clusters of more than 8 are asked for once per kernel and device
+    static bool set[64] = {false};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return LA_ERR_CUDA;
+    if (!set[dev]) {
+      const cudaError_t e =
+          cudaFuncSetAttribute(simt_product_kernel<TILE, PAIR>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) {
+        note_cuda_error(e, "cluster size");
+        return LA_ERR_CUDA;
+      }
+      set[dev] = true;
+    }
+  }
+  return launch_early(simt_product_kernel<TILE, PAIR>, dim3((unsigned)grid), simt_threads<TILE>(), 0, st,
+                      a.splits > 1 ? a.splits : 0, a);
+}
+
+int simt_launch(const Product &p, const SimtPlan &plan, cudaStream_t st) {
   SimtArgs a = {};
   a.M = p.M; a.N = p.N; a.e = p.e;
   for (int s = 0; s < 2; ++s) {
@@ -560,13 +597,10 @@ int simt_launch(const Product &p, const SimtPlan &plan, float *partial, cudaStre
   const int64_t mt = (p.M + plan.tile - 1) / plan.tile;
   a.n_tiles = (int)((p.N + plan.tile - 1) / plan.tile);
   a.splits = plan.splits;
-  a.partial = partial;
   const int64_t grid = mt * a.n_tiles * plan.splits;
   if (grid > INT32_MAX) return LA_ERR_TOO_LARGE;
-  if (plan.tile == 128)
-    return launch_early(simt_product_kernel<128, false>, dim3((unsigned)grid), simt_threads<128>(), 0, st, 0, a);
-  return launch_early(p.pair ? simt_product_kernel<64, true> : simt_product_kernel<64, false>, dim3((unsigned)grid),
-                      simt_threads<64>(), 0, st, 0, a);
+  if (plan.tile == 128) return simt_launch_tile<128, false>(a, grid, st);
+  return p.pair ? simt_launch_tile<64, true>(a, grid, st) : simt_launch_tile<64, false>(a, grid, st);
 }
 
 // Whether a product is few_tokens_fp32_kernel's kind, and the launch: enough warps to fill the GPU, each with 256 terms.
@@ -586,13 +620,6 @@ int few_fp32_launch(const Product &p, cudaStream_t st) {
               *w1 = static_cast<const float *>(p.b[1].p);
   return launch_early(p.pair ? few_tokens_fp32_kernel<MT, true> : few_tokens_fp32_kernel<MT, false>, dim3(grid), 256, 0, st, 0, x,
                       p.a[0].ld, w0, p.b[0].ld, w1, p.b[1].ld, (int)p.M, (int)p.N, (int)p.K[0], share, e);
-}
-
-int split_sum_launch(const Product &p, int splits, const float *partial, cudaStream_t st) {
-  const int64_t grid = (p.M * ((p.N + 7) / 8) + 255) / 256;
-  if (grid > INT32_MAX) return LA_ERR_TOO_LARGE;
-  return launch_early(p.pair ? split_sum_kernel<true> : split_sum_kernel<false>, dim3((unsigned)grid), 256, 0, st, 0, partial,
-                      splits, p.M, (int)p.N, p.e);
 }
 
 // The operand as the tensor cores can read it: itself, or its copy with rows on 16-byte boundaries.
@@ -625,23 +652,18 @@ int product(Product p, int dtype, Scratch s, int64_t &need, cudaStream_t st) {
     if (p.M == 2) return few_fp32_launch<2>(p, st);
     return p.M <= 4 ? few_fp32_launch<4>(p, st) : few_fp32_launch<8>(p, st);
   }
-  GemmPlan plan = {};
-  SimtPlan simt = {};
-  int64_t bytes = 0;
   if (dtype == LA_F32) {
-    simt = simt_plan(p);
-    if (simt.splits > 1) bytes = (int64_t)simt.splits * (p.pair ? 2 : 1) * p.M * p.N * 4;
-  } else {
-    plan = gemm_plan(p.M, p.N, p.K[0], p.segments > 1 ? p.K[1] : 0, p.pair != 0);
-    bytes = plan.partial_bytes;
+    if (s.used > need) need = s.used;
+    if (s.base == nullptr) return LA_OK;
+    p.e.vec = epilogue_vec(p.e, dtype);
+    return simt_launch(p, simt_plan(p), st);
   }
-  float *partial = bytes > 0 ? static_cast<float *>(s.take(bytes)) : nullptr;
+  const GemmPlan plan = gemm_plan(p.M, p.N, p.K[0], p.segments > 1 ? p.K[1] : 0, p.pair != 0);
+  float *partial = plan.partial_bytes > 0 ? static_cast<float *>(s.take(plan.partial_bytes)) : nullptr;
   if (s.used > need) need = s.used;
   if (s.base == nullptr) return LA_OK;
   p.e.vec = epilogue_vec(p.e, dtype);
-  if (dtype != LA_F32) return gemm_launch(p, plan, partial, dtype, st);
-  const int rc = simt_launch(p, simt, partial, st);
-  return rc != LA_OK || partial == nullptr ? rc : split_sum_launch(p, simt.splits, partial, st);
+  return gemm_launch(p, plan, partial, dtype, st);
 }
 
 template <typename T, int VEC>
