@@ -120,10 +120,10 @@ __device__ __forceinline__ void simt_put(bool mn, float (*s)[TILE + 4], const fl
 // One TILE x TILE tile (of one split) per CTA, 8 x 4 results a thread (TILE 64, 128 threads) or 8 x 8 (TILE 128, 256 threads),
 // packed over pairs of rows; the next step's operands are in registers while the current step's are multiplied.  The splits
 // of a tile are a cluster: each CTA adds everyone's sums for a part of the tile, in order, out of shared memory.  2048 x 2048 x
-// 2048 416 us (41 TFLOP/s; the instructions beside the products and shared memory bound it; elements of B kept twice in shared
-// memory, to save doubling them in registers, 860 us).  514 x 512 x 512 14.6 us, 128 x 16384 x 128 57; with the splits' sums
-// through global memory and a second launch 16.7 and 61, but 16 x 4096 x 4096 61 instead of 70 (clusters of 9 fill the SMs
-// less evenly).
+// 2048 402 us (43 TFLOP/s: 256 tiles in 296 places, and shared memory and the instructions beside the products, which leave
+// the multipliers two thirds of their time; elements of B kept twice in shared memory, to save doubling them in registers, 860
+// us).  514 x 512 x 512 14.3 us, 128 x 16384 x 128 52; with the splits' sums through global memory and a second launch 16.7 and
+// 61, but 16 x 4096 x 4096 61 instead of 67 (clusters of 9 fill the SMs less evenly).
 template <int TILE, bool PAIR>
 __global__ void __launch_bounds__(simt_threads<TILE>(), TILE == 128 ? 2 : (PAIR ? 3 : 5)) simt_product_kernel(const SimtArgs a) {
   constexpr int TN = TILE / 16;  // columns a thread: 4 from tx * 4 on, and for TILE 128 4 from 64 + tx * 4 on
@@ -137,7 +137,8 @@ __global__ void __launch_bounds__(simt_threads<TILE>(), TILE == 128 ? 2 : (PAIR 
   __shared__ __align__(16) Shared mem;
   auto &sa = mem.in.a;
   auto &sb = mem.in.b;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  // a warp has 8 x 4 threads' results: fewer bytes out of shared memory than with 16 x 2 (2048 cubed 416 -> 401 us)
+  const int tx = (threadIdx.x >> 5 & 1) * 8 + (threadIdx.x & 7), ty = (threadIdx.x >> 6) * 4 + (threadIdx.x >> 3 & 3);
   const long long tile = blockIdx.x / a.splits;
   const int split = (int)(blockIdx.x - tile * a.splits);
   const long long m0 = tile / a.n_tiles * TILE, n0 = tile % a.n_tiles * TILE;
@@ -541,27 +542,36 @@ int epilogue_vec(const Epilogue &e, int dtype) {
 }
 
 // Tile and splits of an fp32 product.  Tiles of 128 where the result is wider than 64 both ways and they and their splits
-// fill the GPU, else of 64; splits for two (tiles of 128) or four CTAs an SM, of at least 256 or 64 terms.  With tiles of 64 /
-// of 128: 1024 x 1024 x 1024 79 / 59 us, 700 x 2000 x 3000 286 / 202, 16 x 4096 x 4096 70 / 141.
+// fill the GPU, else of 64.  With tiles of 64 / of 128: 1024 x 1024 x 1024 76 / 57 us, 4096 x 1024 x 4096 772 / 679, 16 x 4096 x
+// 4096 67 / 141.  Splits of at least 64 terms for four CTAs of 64 an SM.  Those of 128, two an SM, split into the power of
+// two, of at least 256 terms, that leaves the least of the last round idle: 3.1 us a step of two CTAs, 2.2 of one alone, 4 us a
+// round beside, 10 with the sums (1500 x 768 x 2048 in 1, 2, 4: 156, 120, 122; 4096 x 1024 x 4096 679, 692, 748; three, 133 and 769, do not
+// pack as two CTAs an SM).
 struct SimtPlan {
   int tile, splits;
 };
 SimtPlan simt_plan(const Product &p) {
   const int64_t k = p.K[0] + (p.segments > 1 ? p.K[1] : 0), sms = sm_count();
-  auto plan = [&](int tile, int64_t per_sm, int64_t terms) {
-    const int64_t tiles = (p.M + tile - 1) / tile * ((p.N + tile - 1) / tile);
-    int64_t splits = per_sm * sms / tiles;
-    if (splits > k / terms) splits = k / terms;
-    if (splits > 16) splits = 16;
-    if (splits < 1) splits = 1;
-    return SimtPlan{tile, (int)splits};
-  };
   if (!p.pair && p.M > 64 && p.N > 64) {
-    const SimtPlan big = plan(128, 2, 256);
     const int64_t tiles = (p.M + 127) / 128 * ((p.N + 127) / 128);
-    if (tiles * big.splits >= sms) return big;
+    int best = 1;
+    double best_us = 1e30;
+    for (int s = 1; s <= 8 && (s == 1 || k / s >= 256); s *= 2) {
+      const int64_t rounds = tiles * s / (2 * sms), rest = tiles * s % (2 * sms);
+      const double step = rest == 0 ? 0 : rest <= sms && (rounds > 0 || s == 1) ? 2.2 : 3.1;
+      const double us = (k / kStep / s) * (rounds * 3.1 + step) + (rounds + (rest > 0)) * (s == 1 ? 4 : 10);
+      if (us < best_us) {
+        best_us = us;
+        best = s;
+      }
+    }
+    if (tiles * best >= sms) return SimtPlan{128, best};
   }
-  return plan(64, 4, 64);
+  const int64_t tiles = (p.M + 63) / 64 * ((p.N + 63) / 64);
+  int64_t splits = 4 * sms / tiles;
+  if (splits > k / 64) splits = k / 64;
+  if (splits > 16) splits = 16;
+  return SimtPlan{64, splits < 1 ? 1 : (int)splits};
 }
 
 template <int TILE, bool PAIR>
