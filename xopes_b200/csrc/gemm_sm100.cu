@@ -545,9 +545,12 @@ int launch_t(const Product &p, const GemmArgs &g, int units, cudaStream_t st) {
 }  // namespace
 
 // Estimates the kernel's time for tiles of 256 and 128 columns, whole or split: every tile in s units, or the tiles of the last,
-// incomplete round in as many units as there are pairs for.  A stage takes 0.28 us (256 columns) or 0.20, a tile 0.5 us
-// besides, sums another launch (2.5 us) and their way to memory and back (4 TB/s).  Against measurements of 17 shapes with
-// 1 .. 16 units a tile the estimate's choice was the quickest or within 4 % of it in 15, within 9 % in all.
+// incomplete round in as many units as there are pairs for (tiles of 256 only: whole rounds of narrow ones run at the power
+// limit, where they lose to wide tiles that are all split: dW of a pair, 2 x 2048 x 16384 x 768, 107 .. 112 against 95 us).  A
+// stage takes 0.28 us (256 columns) or 0.20, a tile 0.5 us besides, sums another launch (2.5 us) and their way to memory
+// and back (4 TB/s).  Against measurements of 17 shapes with 1 .. 16 units a tile the estimate's choice was the quickest or
+// within 4 % of it in 15, within 9 % in all.  The last round split: 4096 x 16384 x 4096 387 -> 383 and in another run 378 -> 366 us,
+// 256 tokens through a pair of 11008 x 4096 55 -> 50.
 GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K0, int64_t K1, bool pair) {
   const int64_t pairs = sm_count() / 2;
   const int64_t mt = (M + kRows - 1) / kRows, rows = M < kRows ? M : kRows;
@@ -572,7 +575,7 @@ GemmPlan gemm_plan(int64_t M, int64_t N, int64_t K0, int64_t K1, bool pair) {
     consider(tiles, 1);
     for (int64_t s = 2; s <= 16 && s * 4 <= kb + 3; ++s) {
       if (tiles * (s - 1) < pairs * 4) consider(0, s);
-      if (tiles > pairs && tiles % pairs * s <= pairs) consider(tiles / pairs * pairs, s);
+      if (bn == 256 && tiles > pairs && tiles % pairs * s <= pairs) consider(tiles / pairs * pairs, s);
     }
   }
   return best;
