@@ -292,3 +292,33 @@ def test_offsets_past_32_bits():
     close("dx", dz @ w.double(), dx[-3:], torch.bfloat16, dz.abs() @ w.double().abs(),
           float((e.square() @ w.double().square()).sum().sqrt()))
     assert (dx[:-3] == 0).all()
+
+
+@pytest.mark.parametrize("m,k,n", [(64, 4096, 64), (65, 2050, 67), (200, 1030, 130), (9, 1024, 30), (130, 4096, 1100), (1500, 768, 2048)])
+@pytest.mark.parametrize("pair", [False, True])
+def test_fp32_contraction_shared_by_a_cluster(m, k, n, pair):
+    """Splits of 2 to 16 (clusters above 8 among them), ragged tiles, both tile sizes."""
+    check(m, k, n, torch.float32, "silu", bias=True, residual=not pair, pair=pair)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n,pair", [(300, 2048, 10000, False), (300, 2050, 9992, False), (257, 1024, 10004, True), (1100, 4096, 4100, False)])
+def test_last_round_of_tiles_split(m, k, n, pair, dtype):
+    """A few tiles more than the GPU holds at once: those are split, the others whole."""
+    check(m, k, n, dtype, "gelu", bias=True, residual=not pair, pair=pair)
+
+
+@pytest.mark.parametrize("m,k,n,dtype", [(64, 4096, 64, torch.float32), (300, 2048, 10000, torch.bfloat16)])
+def test_split_sums_repeat_and_replay(m, k, n, dtype):
+    from xopes_b200.linear import linear_fn
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x, w = (torch.randn(*s, generator=g, device="cuda").to(dtype) for s in ((m, k), (n, k)))
+    want = linear_fn(x, w)
+    assert torch.equal(want, linear_fn(x, w))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = linear_fn(x, w)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        assert torch.equal(want, got)
