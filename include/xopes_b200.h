@@ -383,7 +383,8 @@ LA_API int la_qk_norm_rope_bwd(const void *q, int64_t q_sb, int64_t q_sn, int64_
  *     la_gated_linear_fwd  g = x Wg^T + b_gate, u = x Wu^T + b_up;  h = act(g) u
  * z resp. gu receive what the backward reads (pre-activations: fp32, or the upper 24 bits of fp32 for 16-bit types), or
  * are NULL: la_linear_saved_bytes(M, N, dtype, pair) bytes, 16-byte aligned.  Accumulation in fp32, one
- * rounding after the whole epilogue.  16-bit types run on the tensor cores, fp32 on the CUDA cores.
+ * rounding after the whole epilogue.  16-bit types run on the tensor cores, fp32 on the CUDA cores.  fp32 relu keeps values
+ * near 0 as their sums in 64 bits say, since their sign decides the derivative.
  *     la_linear_bwd        dz = d_y act'(z);  dx = dz W, dweight = dz^T x, dbias = sum over rows of dz
  *     la_gated_linear_bwd  dg = d_h u act'(g), du = d_h act(g);  dx = dg Wg + du Wu, dw_* , db_* as above
  * Outputs that are NULL are skipped (dw_gate and dw_up only together).  dz, dg and du are rounded to `dtype`.
