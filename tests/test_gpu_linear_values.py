@@ -53,3 +53,32 @@ def test_relu_border_fp32(pair, m, k, n):
     near("dx", dx, dx64, size @ W.abs() + (up @ v.double().abs() + dy.double().abs() @ v.double().abs() if pair else 0), 2 * n + k)
     near("dw", dw, dz.t() @ X, size.t() @ X.abs(), m + k)
     near("db", db, dz.sum(0), size.sum(0), m + k)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m", [1, 8, 20, 200])
+@pytest.mark.parametrize("pair", [False, True])
+def test_relu_of_small_whole_numbers(pair, m, dtype):
+    """Sums of small whole numbers are exact in fp32, so results and gradients are those in 64 bits, rounded once:
+    many pre-activations are 0, where the derivative is 0, and those of one column are NaN, where the gradient passes."""
+    import torch.nn.functional as F
+    from xopes_b200.linear import gated_linear_fn, linear_fn
+    k, n = 16, 24
+    g = torch.Generator(device="cuda").manual_seed(m)
+    whole = lambda *s: torch.randint(-1, 2, s, generator=g, device="cuda").to(dtype)  # noqa: E731
+    x, w, v, dy, b = whole(m, k), whole(n, k), whole(n, k), whole(m, n), whole(n)
+    b[5] = float("nan")
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    leaves64 = [t.detach().double().requires_grad_() for t in (x, w, b)]
+    z = leaves64[0] @ leaves64[1].t() + leaves64[2]
+    assert int((z == 0).sum()) > 0
+    if pair:
+        y = gated_linear_fn(x, w, v, b, act="relu")
+        y64 = F.relu(z) * (x.detach().double() @ v.double().t())
+        wanted = [1, 2]  # dx takes in du of the NaN column
+    else:
+        y, y64, wanted = linear_fn(x, w, b, act="relu"), F.relu(z), [0, 1, 2]
+    assert torch.equal(torch.nan_to_num(y, nan=-99.0), torch.nan_to_num(y64.to(dtype), nan=-99.0))
+    got, ref = torch.autograd.grad(y, leaves, dy), torch.autograd.grad(y64, leaves64, dy.double())
+    for i in wanted:
+        assert torch.equal(got[i], ref[i].to(dtype)), (i, got[i], ref[i])

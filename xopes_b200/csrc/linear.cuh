@@ -88,7 +88,7 @@ __device__ __forceinline__ void activate_grad(float (&z)[W], float (&d)[W], int 
   if (kind == kActRelu) {
 #pragma unroll
     for (int j = 0; j < W; ++j) {
-      d[j] = z[j] > 0.f ? 1.f : 0.f;
+      d[j] = z[j] <= 0.f ? 0.f : 1.f;  // NaN: the gradient passes, as the value does
       z[j] = z[j] > 0.f || z[j] != z[j] ? z[j] : 0.f;
     }
     return;
