@@ -82,3 +82,39 @@ def test_relu_of_small_whole_numbers(pair, m, dtype):
     got, ref = torch.autograd.grad(y, leaves, dy), torch.autograd.grad(y64, leaves64, dy.double())
     for i in wanted:
         assert torch.equal(got[i], ref[i].to(dtype)), (i, got[i], ref[i])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m", [7, 100, 4000])
+@pytest.mark.parametrize("act", ["gelu", "silu", "sigmoid"])
+def test_activations_over_their_whole_range(act, m, dtype):
+    """Pre-activations that are given (a product with one term, of weight 1), so that every result and gradient stands for one
+    value of the activation or its derivative.  Half a step of the type (in the subnormal range of fp16 2^-25) for the
+    rounding, and for the value 3e-5 of it: exponentials e^a with a rounded two or three times, 2^-24 |a| each, |a| below 90;
+    the normal distribution's tail e^(-z^2 / 2) R(|z|) with R fitted to 5e-6; a few steps of 2^-23.  The derivative is a sum
+    of two such values, and has 1 - s for a sigmoid s, which is off by 2^-24.  It is taken at what the forward kept of z: 24 of
+    32 bits for 16-bit types, the others filled, so off by at most 2^-15 |z| (bits of z below the 15 of the mantissa), which
+    moves the derivative by 2^-15 |z act''(z)|; bf16 has no such bits.  Below 2^-118 nothing is said (1 / x of the
+    special function unit ends at 2^-126)."""
+    import torch.nn.functional as F
+    from xopes_b200.linear import linear_fn
+    top = 13.0 if act == "gelu" else 80.0
+    z = torch.linspace(-top, top, m * 16, device="cuda").to(dtype).view(m, 16).requires_grad_()
+    y = linear_fn(z, torch.eye(16, device="cuda").to(dtype), act=act)
+    dz, = torch.autograd.grad(y, z, torch.ones_like(y))
+    t = z.detach().double()
+    s, phi = torch.sigmoid(t), torch.exp(-0.5 * t * t) * 0.3989422804014327
+    cdf = 0.5 * torch.special.erfc(-t * 0.5 ** 0.5)
+    y64, parts = {"gelu": (t * cdf, (cdf, t * phi)), "silu": (t * s, (s, t * s * torch.sigmoid(-t))),
+                  "sigmoid": (s, (s * torch.sigmoid(-t), 0 * s))}[act]
+    assert torch.allclose(y64, {"gelu": F.gelu, "silu": F.silu, "sigmoid": torch.sigmoid}[act](t), rtol=0, atol=1e-14)
+    floor = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -118
+    half = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype]
+    more = {"gelu": (2 - t * t) * phi, "silu": s * torch.sigmoid(-t) * (2 + t * (1 - 2 * s)),
+            "sigmoid": s * torch.sigmoid(-t) * (1 - 2 * s)}[act].abs() * t.abs() * (2.0 ** -15 if dtype == torch.float16 else 0.0)
+    more = more + (2.0 ** -23 if act == "sigmoid" else 0.0)
+    for name, got, ref, size, more in (("y", y, y64, y64.abs(), 0.0),
+                                       ("dz", dz, parts[0] + parts[1], parts[0].abs() + parts[1].abs(), more)):
+        off = (got.detach().double() - ref).abs() - half * ref.abs() - 3e-5 * size - floor - more
+        worst = int(off.argmax())
+        assert float(off.flatten()[worst]) <= 0, (name, *(float(v.detach().flatten()[worst]) for v in (z, got, ref)))
