@@ -118,3 +118,25 @@ def test_activations_over_their_whole_range(act, m, dtype):
         off = (got.detach().double() - ref).abs() - half * ref.abs() - 3e-5 * size - floor - more
         worst = int(off.argmax())
         assert float(off.flatten()[worst]) <= 0, (name, *(float(v.detach().flatten()[worst]) for v in (z, got, ref)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m", [1, 8, 100, 300])
+@pytest.mark.parametrize("n", [24, 140, 204, 75])
+def test_epilogue_access_widths(n, m, dtype):
+    """Bias and residual on 16 bytes, on 8 and on neither, results of widths that are multiples of 8, of 4 and of neither; whole
+    numbers, whose sums are exact in every type (at most 64 + 2), so that every element is known."""
+    from xopes_b200.linear import gated_linear_fn, linear_fn
+    g = torch.Generator(device="cuda").manual_seed(m + n)
+    whole = lambda *s: torch.randint(-1, 2, s, generator=g, device="cuda").to(dtype)  # noqa: E731
+    x, w, v = whole(m, 64), whole(n, 64), whole(n, 64)
+    biases, wide = whole(n + 8), whole(m, n + 16)
+    z, u = x.double() @ w.double().t(), x.double() @ v.double().t()
+    for at in (0, 8, 4, 1):
+        b, r = biases[at:at + n], wide[:, at:at + n]
+        y = linear_fn(x, w, b, residual=r, act="relu")
+        assert torch.equal(y, ((z + b.double()).clamp(min=0) + r.double()).to(dtype)), at
+        y = linear_fn(x, w, residual=r)
+        assert torch.equal(y, (z + r.double()).to(dtype)), at
+        h = gated_linear_fn(x, w, v, b, biases[:n], act="relu")
+        assert torch.equal(h, ((z + b.double()).clamp(min=0) * (u + biases[:n].double())).to(dtype)), at

@@ -7,8 +7,9 @@
 // a ring of TMA boxes, leaves its sums in its shared memory, and finishes a part of the tokens by adding up the sums of
 // all S through distributed shared memory, in order.  One launch, no scratch, equal calls give equal bits.
 //
-// Bound by HBM: 64 tokens through 2 x 11008 rows of 4096 (bf16) are 27.6 us at the measured copy bandwidth; 33.8 here, 49.7
-// with 256-token tiles and a second kernel for the splits of the contraction.  1 token, 4096 rows of 4096: 5.1, 9.2, 17.6.
+// Bound by HBM: 64 tokens through 2 x 11008 rows of 4096 (bf16) are 27.6 us at the measured copy bandwidth; 35 .. 37 here, 50
+// with 256-token tiles and a second kernel for the splits of the contraction.  1 token, 4096 rows of 4096: 5.1, 9.5, 17.6.
+// The epilogue's rows in accesses of 8 bytes: 128 tokens through 4096 x 4096 17.6 -> 17.4 us, through 8192 x 1024 14.75 -> 14.5.
 // What is left there is the launch, the first loads' way and the two cluster barriers; at 64 tokens the tokens' own boxes, which
 // every CTA reads from L2, take half of what the weights take.
 #include "linear.cuh"

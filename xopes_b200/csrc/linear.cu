@@ -719,6 +719,7 @@ int readable(Operand &o, int64_t rows, int64_t cols, int dtype, Scratch &s, cuda
 
 // One product with its epilogue.  With s.base null only the scratch is counted.
 int product(Product p, int dtype, Scratch s, int64_t &need, cudaStream_t st) {
+  p.e.vec = epilogue_vec(p.e, dtype);
   if (few_tokens_fit(p, dtype)) {
     if (s.used > need) need = s.used;
     return s.base == nullptr ? LA_OK : few_tokens_launch(p, dtype, st);
@@ -733,14 +734,12 @@ int product(Product p, int dtype, Scratch s, int64_t &need, cudaStream_t st) {
   if (dtype == LA_F32) {
     if (s.used > need) need = s.used;
     if (s.base == nullptr) return LA_OK;
-    p.e.vec = epilogue_vec(p.e, dtype);
     return simt_launch(p, simt_plan(p), st);
   }
   const GemmPlan plan = gemm_plan(p.M, p.N, p.K[0], p.segments > 1 ? p.K[1] : 0, p.pair != 0);
   float *partial = plan.partial_bytes > 0 ? static_cast<float *>(s.take(plan.partial_bytes)) : nullptr;
   if (s.used > need) need = s.used;
   if (s.base == nullptr) return LA_OK;
-  p.e.vec = epilogue_vec(p.e, dtype);
   return gemm_launch(p, plan, partial, dtype, st);
 }
 
