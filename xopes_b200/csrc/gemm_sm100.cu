@@ -66,19 +66,21 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// the same barrier in the first CTA of the pair
-__device__ __forceinline__ void arrive_first(uint32_t bar) {
-  asm volatile(
-      "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, 0;\n\t"
-      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n\t}" ::"r"(bar) : "memory");
+// the same place in the first CTA of the pair
+__device__ __forceinline__ uint32_t in_first(uint32_t addr) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
 }
-// a box into this CTA's shared memory; the bytes count on the first CTA's barrier (bit 24 of a shared-memory address is
-// the CTA's place in the pair)
+__device__ __forceinline__ void arrive_first(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_first(bar)) : "memory");
+}
+// a box into this CTA's shared memory; the bytes count on the first CTA's barrier (`bar`: out of in_first)
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
       " [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar & 0xFEFFFFFFu), "r"(c0), "r"(c1)
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
       : "memory");
 }
 __device__ __forceinline__ void mma_two(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -306,6 +308,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
       prefetch_tmap(&g.a[0]);
       prefetch_tmap(&g.b[PAIR ? rank : 0]);
     }
+    const uint32_t full0 = in_first(full);
     int it = 0;
     bool ok = true;
     for (int u = first; u < units && ok; u += stride) {
@@ -320,9 +323,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gemm_ke
         const int seg = kb >= g.kb[0];
         const int k = (seg ? kb - g.kb[0] : kb) * kStepK;
         const CUtensorMap *ma = &g.a[seg], *mb = &g.b[PAIR ? rank : seg];
-        const uint32_t as = base + s * C::kStage, bs = as + kABytes, bar = full + 8 * s;
+        const uint32_t as = base + s * C::kStage, bs = as + kABytes, bar = full0 + 8 * s;
         if (elect_one()) {
-          if (rank == 0) mbar_arrive_expect_tx(bar, 2 * C::kStage);
+          if (rank == 0) mbar_arrive_expect_tx(full + 8 * s, 2 * C::kStage);
           if (!A_MN) {
             load_box(as, ma, bar, k, am);
           } else {
