@@ -375,11 +375,7 @@ template <> struct RawKept<float, 4> {
 };
 template <typename T> struct RawKept<T, 1> {
   float r;
-  __device__ __forceinline__ void load(const Saved &s, long long off) {
-    float v[1];
-    load_saved<T, 1>(s, off, false, 1, v);
-    r = v[0];
-  }
+  __device__ __forceinline__ void load(const Saved &s, long long off) { r = kept_value<T>(s, off); }
   __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = r; }
 };
 

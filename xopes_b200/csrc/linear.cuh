@@ -268,24 +268,10 @@ __device__ __forceinline__ void kept_values(const uint4 &h4, const uint2 &l2, fl
   for (int j = 0; j < 8; ++j)
     v[j] = __uint_as_float(__byte_perm(l[j / 4], h[j / 2], (j % 4) * 0x11 + (j % 2 ? 0x7600 : 0x5400)));
 }
-template <typename T, int W>
-__device__ __forceinline__ void load_saved(const Saved &s, long long off, bool vec, int left, float (&v)[W]) {
-  if constexpr (sizeof(T) == 4) {
-    load_row<float, W>(static_cast<const float *>(s.p) + off, vec, left, v);
-  } else {
-    const uint16_t *hi = static_cast<const uint16_t *>(s.p) + off;
-    const uint8_t *lo = s.low + off;
-    if constexpr (W % 8 == 0) {
-      if (vec && left >= W) {
-#pragma unroll
-        for (int i = 0; i < W; i += 8)
-          kept_values(*reinterpret_cast<const uint4 *>(hi + i), *reinterpret_cast<const uint2 *>(lo + i), v + i);
-        return;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < W; ++j) v[j] = j < left ? __uint_as_float((uint32_t)hi[j] << 16 | (uint32_t)lo[j] * 0x101u) : 0.f;
-  }
+// one kept value, with the same filling
+template <typename T> __device__ __forceinline__ float kept_value(const Saved &s, long long off) {
+  if constexpr (sizeof(T) == 4) return static_cast<const float *>(s.p)[off];
+  else return __uint_as_float((uint32_t)static_cast<const uint16_t *>(s.p)[off] << 16 | (uint32_t)s.low[off] * 0x101u);
 }
 
 template <typename T, int W>
