@@ -140,3 +140,43 @@ def test_epilogue_access_widths(n, m, dtype):
         assert torch.equal(y, (z + r.double()).to(dtype)), at
         h = gated_linear_fn(x, w, v, b, biases[:n], act="relu")
         assert torch.equal(h, ((z + b.double()).clamp(min=0) * (u + biases[:n].double())).to(dtype)), at
+
+
+def same_kind(name, got, ref, rows=slice(None)):
+    """NaN where ref (64 bits) has NaN, the same infinities, and numbers elsewhere."""
+    got, ref = got.double()[rows], ref[rows]
+    for f in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(f(got), f(ref)), (name, f.__name__, (f(got) != f(ref)).nonzero()[:4].tolist())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m", [6, 70, 300])
+@pytest.mark.parametrize("act", ["none", "relu", "sigmoid", "silu", "gelu"])
+@pytest.mark.parametrize("pair", [False, True])
+def test_infinities_and_not_a_number(pair, act, m, dtype):
+    """A token with an infinity and one with NaN: what becomes of them is what the formulas in 64 bits make of them, forward and in
+    the gradients, and the other tokens' results have the bits that they have without."""
+    import torch.nn.functional as F
+    from xopes_b200.linear import gated_linear_fn, linear_fn
+    fn64 = {"none": lambda t: t, "relu": F.relu, "sigmoid": torch.sigmoid, "silu": lambda t: t * torch.sigmoid(t),
+            "gelu": lambda t: t * 0.5 * torch.special.erfc(-t * 0.5 ** 0.5)}[act]
+    torch.manual_seed(m)
+    x, w, v, dy = (torch.randn(*s, device="cuda").to(dtype) for s in ((m, 72), (48, 72), (48, 72), (m, 48)))
+
+    def run(x):
+        leaves = [t.clone().requires_grad_() for t in (x, w)]
+        y = gated_linear_fn(leaves[0], leaves[1], v, act=act) if pair else linear_fn(*leaves, act=act)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    clean = run(x)
+    x[2, 5], x[m - 2, 71] = float("inf"), float("nan")
+    got = run(x)
+    X, W = x.double().requires_grad_(), w.double().requires_grad_()
+    z = X @ W.t()
+    y64 = fn64(z) * (X @ v.double().t()) if pair else fn64(z)
+    dx64, dw64 = torch.autograd.grad(y64, (X, W), dy.double())
+    others = torch.ones(m, dtype=torch.bool, device="cuda")
+    others[2] = others[m - 2] = False
+    assert torch.equal(got[0][others], clean[0][others]) and torch.equal(got[1][others], clean[1][others])
+    same_kind("y", got[0], y64.detach())
+    same_kind("dx", got[1], dx64)
+    same_kind("dw", got[2], dw64)
