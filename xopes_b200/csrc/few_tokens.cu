@@ -215,7 +215,9 @@ __global__ void __launch_bounds__(kThreads) few_tokens_kernel(const __grid_const
 // run there.  Measured with sizes 1 .. 8 in us, 1 token: 172 tiles of K 4096 32.5 31.3 34 34 37 37 40 39 (2 taken), 96 tiles 22.2
 // 20.4 19.3 19.4 23 23 24 23 (4), 64 tiles of K 8192 35 26 24.4 23.6 23.5 23.8 29 28 (6), 32 tiles of K 4096 19 12 10.3 10.3 9.7 9.6
 // 9.8 9.2 (8); 128 tokens, 32 tiles of K 4096: 32 21 17.7 14.5 16.3 16.0 17.9 17.7 (4), 16 tiles of K 2048: 23 16 13 10.3 10.6
-// 10.9 11.1 9.7 (8); 32 tokens, 32 tiles of K 768: 7.7 5.8 5.8 5.5 6.3 6.5 6.6 7.0 (4).
+// 10.9 11.1 9.7 (8); 32 tokens, 32 tiles of K 768: 7.7 5.8 5.8 5.5 6.3 6.5 6.6 7.0 (4).  Up to 4 against up to 8 CTAs, 64 and 128
+// tokens, K 1024 .. 8192: 32 to 64 tiles 3 .. 20 % less (one of 32 shapes 4 % more), from 80 tiles on no more than 4 fit, 16 and 24 tiles
+// 8 % less at K 1024, up to 11 % more at 8192.
 template <typename T, int MT, bool PAIR>
 int launch_cfg(FewArgs g, int tiles, cudaStream_t st) {
   typedef Cfg<MT> C;

@@ -549,8 +549,9 @@ int launch_t(const Product &p, const GemmArgs &g, int units, cudaStream_t st) {
 
 // Estimates the kernel's time for tiles of 256 and 128 columns, whole or split: every tile in s units, or the tiles of the last,
 // incomplete round in as many units as there are pairs for (tiles of 256 only: whole rounds of narrow ones run at the power
-// limit, where they lose to wide tiles that are all split: dW of a pair, 2 x 2048 x 16384 x 768, 107 .. 112 against 95 us).  A
-// stage takes 0.28 us (256 columns) or 0.20, a tile 0.5 us besides, sums another launch (2.5 us) and their way to memory
+// limit and move more operands: with them 44 products in which they would be taken, which is 1 in 36 of a grid of sizes, needed 2 %
+// more on average; as results 0.85 .. 1.10 of the time, 2 % less, as dW 0.87 .. 1.21, 2 % more, as dx 0.94 .. 1.43, 6 % more).
+// A stage takes 0.28 us (256 columns) or 0.20, a tile 0.5 us besides, sums another launch (2.5 us) and their way to memory
 // and back (4 TB/s).  Against measurements of 17 shapes with 1 .. 16 units a tile the estimate's choice was the quickest or
 // within 4 % of it in 15, within 9 % in all.  The last round split: 4096 x 16384 x 4096 387 -> 383 and in another run 378 -> 366 us,
 // 256 tokens through a pair of 11008 x 4096 55 -> 50.
