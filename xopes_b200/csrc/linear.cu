@@ -490,9 +490,9 @@ __global__ void __launch_bounds__(256) bias_sum_kernel(const float *partial, int
 // So the kept values near 0 are computed again in 64 bits.  Near: each of the sum's K roundings is at most 2^-24 |x_m| |w_n|,
 // since no partial sum is above |x_m| |w_n|; with independent signs they add up to sqrt(K) of that, and six times as much is
 // taken: for normally distributed values a share of 3e-7 K of the elements.  Only the derivative reads what is kept, so a
-// forward without gradients has no such pass.  16-bit types do without: of 20 million values 6 are on the other side at K 2048 and 31 at
-// 8192, which moves their gradients by far less in norm than the rounding of dz does, and another pass over z, x and W would cost
-// a tenth of the forward's time.  Forward that keeps its values, relu / sigmoid: 514 x 512 x 512 19.2 / 14.6 us, 1024 x 4096 x 4096 846 / 786
+// forward without gradients has no such pass.  16-bit types do without: on the tensor cores 6 of 20 million values are on the
+// other side at K 2048 and 31 at 8192, and the passes that find and mend them were built and cost more than they are worth there
+// (16384 x 4096 x 4096 390 -> 500 us, 16384 x 768 x 2048 60 -> 90, 1024 x 4096 x 4096 31 -> 54).  Forward that keeps its values, relu / sigmoid: 514 x 512 x 512 19.2 / 14.6 us, 1024 x 4096 x 4096 846 / 786
 // (23 without a value near 0), 8 x 4096 x 4096 39 / 21.
 //
 // near_zero[m] = 6 sqrt(K) 2^-24 |x_m|, near_zero[M + n] = |w_n| (rows of values so far from 1 that their squares leave the
