@@ -10,8 +10,8 @@
 // the pair and residual.  What the backward needs of the forward is z, or g and u: for 16-bit types kept as the upper 24
 // bits of their fp32 values (computing them again would cost a third of the forward's and backward's products together; kept
 // in 16 bits their two roundings made the gradients of a pair 1.8 times as far off as rounding the gradients alone
-// does, in 24 bits 1.4 times, which is what the rounding of dz leaves).  dz is rounded to the type of x, since it is an
-// operand of two products.
+// does, in 24 bits 1.42 times, which is what the rounding of dz leaves).  dz, dg and du are rounded to the type of x, since they are
+// operands of two products; in fp16 one above 65504 becomes infinite, as a loss scale has to see to.
 #include "linear.cuh"
 
 namespace la {
@@ -492,8 +492,9 @@ __global__ void __launch_bounds__(256) bias_sum_kernel(const float *partial, int
 // taken: for normally distributed values a share of 3e-7 K of the elements.  Only the derivative reads what is kept, so a
 // forward without gradients has no such pass.  16-bit types do without: on the tensor cores 6 of 20 million values are on the
 // other side at K 2048 and 31 at 8192, and the passes that find and mend them were built and cost more than they are worth there
-// (16384 x 4096 x 4096 390 -> 500 us, 16384 x 768 x 2048 60 -> 90, 1024 x 4096 x 4096 31 -> 54).  Forward that keeps its values, relu / sigmoid: 514 x 512 x 512 19.2 / 14.6 us, 1024 x 4096 x 4096 846 / 786
-// (23 without a value near 0), 8 x 4096 x 4096 39 / 21.
+// (16384 x 4096 x 4096 390 -> 500 us, 16384 x 768 x 2048 60 -> 90, 1024 x 4096 x 4096 31 -> 54).
+// Forward that keeps its values, relu / sigmoid: 514 x 512 x 512 19.2 / 14.6 us, 1024 x 4096 x 4096 846 / 786 (810 if no value is
+// near 0), 8 x 4096 x 4096 39 / 21.
 //
 // near_zero[m] = 6 sqrt(K) 2^-24 |x_m|, near_zero[M + n] = |w_n| (rows of values so far from 1 that their squares leave the
 // range of fp32 are not looked at).  A warp a row, every operand once: HBM or L2.

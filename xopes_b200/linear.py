@@ -200,9 +200,12 @@ def linear_fn(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor
     """y = act(x weight^T + bias) + residual, in one kernel.
 
     x (..., K), weight (N, K), bias (N), residual (..., N), all of one dtype; rows may be strided (slices need no copy; rows
-    of 16-bit tensors that do not start on 16 bytes, as with odd widths, are copied first).
-    act: "none", "relu", "sigmoid", "silu" or "gelu" (the exact one, by erf).  The backward keeps x, the weight and,
-    with an activation, the pre-activation (24 bits a value, fp32: 32)."""
+    of 16-bit tensors that do not start on 16 bytes, as with odd widths, are copied first, and so is a tensor whose features
+    are not next to each other, such as a transposed weight, forward and backward).
+    act: "none", "relu", "sigmoid", "silu" or "gelu" (the exact one, by erf).  relu's derivative is 0 at 0 and 1 at NaN; in
+    fp32 the exact sum decides which side of 0 a value is on, in 16-bit types the fp32 sum.  The backward keeps x, the weight
+    and, with an activation, the pre-activation (24 bits a value, fp32: 32), and rounds its gradient to x's dtype.
+    Differentiable once: create_graph=True raises RuntimeError."""
     _check_bias(bias, weight.shape[0])
     if residual is not None and residual.shape != (*x.shape[:-1], weight.shape[0]):
         raise ValueError(f"residual must have shape {(*x.shape[:-1], weight.shape[0])}, got {tuple(residual.shape)}")
