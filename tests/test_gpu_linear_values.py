@@ -180,3 +180,40 @@ def test_infinities_and_not_a_number(pair, act, m, dtype):
     same_kind("y", got[0], y64.detach())
     same_kind("dx", got[1], dx64)
     same_kind("dw", got[2], dw64)
+
+
+def test_relu_border_in_a_graph_and_on_two_streams():
+    """What is near 0 is found anew in every replay, and calls side by side have room of their own for it."""
+    from xopes_b200.linear import gated_linear_fn, linear_fn
+    m, k, n = 90, 260, 130
+    torch.manual_seed(0)
+
+    def data():
+        x, w = torch.randn(m, k, device="cuda"), torch.randn(n, k, device="cuda") * k ** -0.5
+        z = x.double() @ w.double().t()
+        return x, w, -z[torch.arange(n, device="cuda") % m, torch.arange(n, device="cuda")].float()
+
+    def step(x, w, b, dy):
+        x, w, b = (t.detach().requires_grad_() for t in (x, w, b))
+        y, h = linear_fn(x, w, b, act="relu"), gated_linear_fn(x, w, w, b, act="relu")
+        return [y.detach(), h.detach(), *torch.autograd.grad((y, h), (x, w, b), (dy, dy))]
+    sets, dy = [data() for _ in range(3)], torch.randn(m, n, device="cuda")
+    refs = [step(*s, dy) for s in sets]
+    place = [torch.empty_like(t) for t in sets[0]]
+    for p, t in zip(place, sets[0]):
+        p.copy_(t)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*place, dy)
+    for s, ref in zip(sets, refs):
+        for p, t in zip(place, s):
+            p.copy_(t)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(ref, got))
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(step(*sets[i % 3], dy))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for i, out in enumerate(outs) for a, b in zip(refs[i % 3], out))

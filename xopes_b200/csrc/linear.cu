@@ -609,10 +609,10 @@ int epilogue_vec(const Epilogue &e, int dtype) {
 
 // Tile and splits of an fp32 product.  Tiles of 128 where the result is wider than 64 both ways and they and their splits
 // fill the GPU, else of 64.  With tiles of 64 / of 128: 1024 x 1024 x 1024 76 / 57 us, 4096 x 1024 x 4096 772 / 679, 16 x 4096 x
-// 4096 67 / 141.  Splits of at least 64 terms for four CTAs of 64 an SM, those of a pair by pair_splits.  Those of 128, two an SM, split into the power of
-// two, of at least 256 terms, that leaves the least of the last round idle: 3.1 us a step of two CTAs, 2.2 of one alone, 4 us a
-// round beside, 10 with the sums (1500 x 768 x 2048 in 1, 2, 4: 156, 120, 122; 4096 x 1024 x 4096 679, 692, 748; three, 133 and 769, do not
-// pack as two CTAs an SM).
+// 4096 67 / 141.  Splits of at least 64 terms for four CTAs of 64 an SM (five fit: 30 shapes 3 % behind the quickest of 1 .. 16
+// splits on average), those of a pair by pair_splits.  Those of 128, two an SM, split into the power of two, of at least 256 terms,
+// that leaves the least of the last round idle: 3.1 us a step of two CTAs, 2.2 of one alone, 4 us a round beside, 10 with the
+// sums (1500 x 768 x 2048 in 1, 2, 4: 156, 120, 122; 4096 x 1024 x 4096 679, 692, 748; three, 133 and 769, do not pack as two CTAs an SM).
 struct SimtPlan {
   int tile, splits;
 };
